@@ -127,9 +127,9 @@ def _to_eight(y):
     blocks = (dim + BLOCK - 1) // BLOCK
     b = torch.nn.functional.pad(y, (0, blocks * BLOCK - dim)).view(n, blocks, BLOCK)
     a = b.abs().amax(2).float()
-    held = a >= TINY
-    scales = torch.where(held, a / 127, 0.0)
-    up = torch.where(held, 127 / a, 0.0)
+    held, top = a >= TINY, torch.full_like(a, 127)  # (by a number, a quotient would be a product with the rounded reciprocal)
+    scales = torch.where(held, a / top, 0.0)
+    up = torch.where(held, top / a, 0.0)
     return torch.round(b.double() * up.double().unsqueeze(2)), scales
 
 
@@ -218,12 +218,12 @@ def work(case):
 
 
 def _exact_eight(y):
-    """What the 8-bit form of 64-bit rows stands for: block after block, scale held in 32 bits."""
+    """What the 8-bit form of 64-bit rows stands for: block after block, largest magnitude and both factors held in 32 bits."""
     out = torch.empty_like(y)
     for c in range(0, y.shape[1], BLOCK):
         b = y[:, c:c + BLOCK]
-        a = b.abs().max(1, keepdim=True).values.float()
-        up, scale = (127 / a).double(), (a / 127).double()
+        a = b.abs().max(1, keepdim=True).values.float().double()
+        up, scale = (127 / a).float().double(), (a / 127).float().double()
         out[:, c:c + BLOCK] = torch.where(a >= TINY, torch.round(b * up) * scale, 0.0)
     return out
 
