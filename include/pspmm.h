@@ -383,6 +383,63 @@ PSPMM_API int pspmm_dense_mm_stalled(int32_t transA, int32_t transB, int64_t M, 
 PSPMM_API int pspmm_dense_status(int32_t *status);
 
 /*
+ * Operators around the layers.  They have no counterpart in the reference, whose features come in as a dense array and whose
+ * layers keep their inputs.  `dtype` names the element type of the arrays passed as void*; sums are in 32 bits or more whatever it is.
+ * Arrays are row-major with a leading dimension in elements; rows that start on 16 bytes are moved by 16-byte loads, others (odd
+ * widths, views) by narrower ones.
+ */
+#define PSPMM_F32 0
+#define PSPMM_BF16 1
+#define PSPMM_F16 2
+
+/*
+ * Rows in 8 bits: per row and block of 128 columns (the last one may be narrower) with largest magnitude a,
+ *     scale = a / 127,   q = rint(x * (127 / a)),   and q * scale stands for x.
+ * A block whose a is below 2^-119 is held as zeros (scale 0); one that holds an infinity or a NaN comes back as NaN throughout.
+ * q[n, pitch]: pitch a multiple of 16 and q 16-byte aligned; the columns from dim to the next multiple of 16 become zeros.
+ * scales[n, ceil(dim / 128)].
+ */
+PSPMM_API int pspmm_quantize_rows(const void *x, int32_t dtype, int64_t ldx, int64_t n, int32_t dim, int8_t *q, int64_t pitch,
+                                  float *scales, void *stream);
+PSPMM_API int pspmm_dequantize_rows(const int8_t *q, int64_t pitch, const float *scales, int32_t dtype, void *out, int64_t ld_out,
+                                    int64_t n, int32_t dim, void *stream);
+
+/*
+ * Root-mean-square norm with the residual's addition:
+ *     h = x + residual,   rstd = (mean(h^2) + eps)^-1/2,   y = h * rstd * weight   (relu != 0: negative y become 0)
+ * residual may be NULL (h = x).  h and y may each be NULL: not wanted.  rstd[n] is always written.  q / scales (both or
+ * neither): y in the 8-bit form above, computed from h, rstd and y in 64 bits.
+ * Backward, from h as stored and rstd:  with g = dy * weight (0 where relu cut) and m = h * rstd,
+ *     dx = rstd * (g - m * mean(g * m)) + dh   (the gradient of x and of residual; dh, the one that reaches h itself, may be NULL)
+ *     dweight = sum over rows of dy * m (0 where relu cut), in an order that depends on the sizes alone.
+ * dx may be dh.  Scratch: pspmm_rms_norm_backward_scratch_bytes, 4-byte aligned.  n == 0 gives a dweight of zeros.
+ */
+PSPMM_API int pspmm_rms_norm(const void *x, int64_t ld_x, const void *residual, int64_t ld_residual, const void *weight,
+                             int32_t dtype, int64_t n, int32_t dim, double eps, int32_t relu, void *h, int64_t ld_h, void *y,
+                             int64_t ld_y, float *rstd, int8_t *q, int64_t pitch, float *scales, void *stream);
+PSPMM_API int pspmm_rms_norm_backward_scratch_bytes(int64_t n, int32_t dim, size_t *bytes);
+PSPMM_API int pspmm_rms_norm_backward(const void *dy, int64_t ld_dy, const void *h, int64_t ld_h, const float *rstd,
+                                      const void *weight, const void *dh, int64_t ld_dh, int32_t dtype, int64_t n, int32_t dim,
+                                      int32_t relu, void *dx, int64_t ld_dx, void *dweight, void *scratch, size_t scratch_bytes,
+                                      void *stream);
+
+/*
+ * Rows of table[n_rows, dim] by id:   out[i] = scale * table[ids[i]],   and the table's gradient from that of out:
+ *     out[t] = scale * sum over {i : ids[i] = t, t != padding} grad[i]        (every row of out is written; padding -1: none)
+ * ids are int64 (ids64 != 0) or int32.  An id outside 0 .. n_rows-1 gives a row of NaN and adds to no gradient, and
+ * pspmm_embedding_status returns 1 from then on in this process (it synchronises).  The sums run over the ids in the order of
+ * their positions, cut at places that depend on n alone: equal calls give equal bits.
+ * The gradient takes at most 2^31 - 65537 ids and needs pspmm_embedding_grad_scratch_bytes(n, dim) bytes, 16-byte aligned.
+ */
+PSPMM_API int pspmm_embedding(const void *ids, int32_t ids64, int64_t n, const void *table, int32_t dtype, int64_t n_rows,
+                              int32_t dim, int64_t ld_table, float scale, void *out, int64_t ld_out, void *stream);
+PSPMM_API int pspmm_embedding_grad_scratch_bytes(int64_t n, int32_t dim, size_t *bytes);
+PSPMM_API int pspmm_embedding_grad(const void *ids, int32_t ids64, int64_t n, const void *grad, int32_t dtype, int64_t ld_grad,
+                                   int64_t n_rows, int32_t dim, float scale, int64_t padding, void *out, int64_t ld_out,
+                                   void *scratch, size_t scratch_bytes, void *stream);
+PSPMM_API int pspmm_embedding_status(int32_t *status);
+
+/*
  * Host-side CSR -> V x 1 block CSR, laid out exactly as scipy's tobsr((V,1)) (which the
  * reference calls at graph_input.py:245-266): blocks of a block-row appear in order of first
  * encounter while walking its V rows top to bottom.  pspmm_bcsr_count fills rowPtr_b

@@ -117,6 +117,18 @@ _SIGNATURES = {
     "pspmm_dense_mm": [_i32, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, ctypes.c_size_t, _vp],
     "pspmm_dense_mm_stalled": [_i32, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, ctypes.c_size_t, _vp],
     "pspmm_dense_status": [ctypes.POINTER(ctypes.c_int32)],
+    "pspmm_quantize_rows": [_vp, _i32, _i64, _i64, _i32, _vp, _i64, _vp, _vp],
+    "pspmm_dequantize_rows": [_vp, _i64, _vp, _i32, _vp, _i64, _i64, _i32, _vp],
+    "pspmm_rms_norm": [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, ctypes.c_double, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _i64,
+                       _vp, _vp],
+    "pspmm_rms_norm_backward_scratch_bytes": [_i64, _i32, ctypes.POINTER(ctypes.c_size_t)],
+    "pspmm_rms_norm_backward": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _i64, _vp, _vp,
+                                ctypes.c_size_t, _vp],
+    "pspmm_embedding": [_vp, _i32, _i64, _vp, _i32, _i64, _i32, _i64, ctypes.c_float, _vp, _i64, _vp],
+    "pspmm_embedding_grad_scratch_bytes": [_i64, _i32, ctypes.POINTER(ctypes.c_size_t)],
+    "pspmm_embedding_grad": [_vp, _i32, _i64, _vp, _i32, _i64, _i64, _i32, ctypes.c_float, _i64, _vp, _i64, _vp, ctypes.c_size_t,
+                             _vp],
+    "pspmm_embedding_status": [ctypes.POINTER(ctypes.c_int32)],
     "pspmm_bcsr_count": [_vp, _vp, _i64, _i64, _i32, _vp, ctypes.POINTER(_i64)],
     "pspmm_bcsr_fill": [_vp, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp],
     "pspmm_mtx_info_read": [ctypes.c_char_p, ctypes.POINTER(MtxInfo)],

@@ -1,0 +1,638 @@
+// Root-mean-square norm of a residual stream, forward and backward:
+//     h = x + r,   rstd = (mean_j h_j^2 + eps)^-1/2,   y_j = h_j rstd w_j   (relu: negative y become 0)
+//     g = dy w [y > 0],   n = h rstd,   dx = rstd (g - n mean_j(g_j n_j)) + dh,   dw_j = sum over rows of dy_j [y > 0] n_j
+// and, where asked for, y in 8 bits (rows8.cu's form) from the same pass.
+//
+// Bound by HBM: every array is moved once.  A row is held in the registers of its lanes between the sum and its use: 8, 16 or
+// 32 lanes (several rows per warp) with up to 16 values each, a CTA of 64 to 1,024 threads beyond that, and two passes over a row
+// wider than 8,192 columns.
+//
+// Numbers: the sum x + r is formed in 32 bits and the squares are added in 64 (which costs nothing here: about six 64-bit
+// operations per value where the memory system leaves time for twenty).  Where y leaves in 8 bits, h, rstd and y are in 64 bits throughout,
+// because next to a half the last bit of a 32-bit y decides which whole number it becomes.  rstd is kept in 32 bits for the backward,
+// whose sums are in 32 bits.
+#include <type_traits>
+
+#include "feature_types.cuh"
+
+namespace {
+using namespace feat;
+
+struct NormArgs {
+    const void *x, *r, *w;
+    void *h, *y;      // either may be null
+    float *rstd;
+    int8_t *q;        // null: no 8-bit form
+    float *scales;
+    int64_t n, ld_x, ld_r, ld_h, ld_y;
+    double eps;
+    int32_t dim, pitch, blocks, relu;
+};
+
+struct NormBackArgs {
+    const void *dy, *h, *w, *dh;  // dh may be null
+    const float *rstd;
+    void *dx;
+    float *part;      // [grid][dim]
+    int64_t n, ld_dy, ld_h, ld_dh, ld_dx;
+    int32_t dim, relu;
+};
+
+struct WeightArgs {
+    const float *part;
+    void *dw;
+    int32_t parts, dim, dtype;
+};
+
+// TPR threads share a row; each holds VPT vectors of VW values.
+template <int TPR> struct Rows {
+    static constexpr int THREADS = TPR <= 32 ? 256 : TPR;
+    static constexpr int PER_CTA = THREADS / TPR;
+    static constexpr int LANES = TPR < 32 ? TPR : 32;  // of a warp that share a row
+};
+
+// Column of a thread's vector v: a warp's lanes side by side, a warp's vectors behind one another (so that the 128 columns of
+// a scale never leave a warp).
+template <int VW, int TPR, int VPT> __device__ __forceinline__ int column(int t, int v)
+{
+    constexpr int L = Rows<TPR>::LANES;
+    return ((t / L * VPT + v) * L + t % L) * VW;
+}
+
+template <typename T, int VW> __device__ __forceinline__ void load_some(float (&f)[VW], const T *p, bool in)
+{
+    if (in) {
+        load_vec<T, VW>(f, p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VW; ++i)
+            f[i] = 0.f;
+    }
+}
+
+template <typename S, int LANES> __device__ __forceinline__ S lanes_sum(S v, uint32_t mask)
+{
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1)
+        v += __shfl_xor_sync(mask, v, d);
+    return v;
+}
+
+// Sum over a row's threads; `sums` has a place per warp and is used again from call to call (two barriers).
+template <typename S, int TPR> __device__ __forceinline__ S row_sum(S v, uint32_t mask, S *sums)
+{
+    v = lanes_sum<S, Rows<TPR>::LANES>(v, mask);
+    if constexpr (TPR > 32) {
+        __syncthreads();
+        if (threadIdx.x % 32 == 0)
+            sums[threadIdx.x / 32] = v;
+        __syncthreads();
+        v = 0;
+#pragma unroll
+        for (int i = 0; i < TPR / 32; ++i)
+            v += sums[i];
+    }
+    return v;
+}
+
+__device__ __forceinline__ uint32_t group_mask(int lanes)
+{
+    return lanes == 32 ? PSPMM_FULL_MASK : ((1u << lanes) - 1) << (threadIdx.x % 32 / lanes * lanes);
+}
+
+template <typename T, int VW, int TPR, int VPT, bool EIGHT>
+__global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs a)
+{
+    using R = Rows<TPR>;
+    using H = typename std::conditional<EIGHT, double, float>::type;
+    __shared__ double sums[R::THREADS / 32];
+    const int t = threadIdx.x % TPR;
+    const uint32_t mask = group_mask(R::LANES);
+    float w[VPT][VW];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        const int c = column<VW, TPR, VPT>(t, v);
+        load_some<T, VW>(w[v], static_cast<const T *>(a.w) + c, c < a.dim);
+    }
+    for (int64_t row = (int64_t)blockIdx.x * R::PER_CTA + threadIdx.x / TPR; row < a.n; row += (int64_t)gridDim.x * R::PER_CTA) {
+        float x[VPT][VW], r[VPT][VW];
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int c = column<VW, TPR, VPT>(t, v);
+            load_some<T, VW>(x[v], static_cast<const T *>(a.x) + row * a.ld_x + c, c < a.dim);
+        }
+        if (a.r) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                const int c = column<VW, TPR, VPT>(t, v);
+                load_some<T, VW>(r[v], static_cast<const T *>(a.r) + row * a.ld_r + c, c < a.dim);
+            }
+        }
+        H h[VPT][VW];
+        double ss = 0;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                h[v][i] = a.r ? (H)x[v][i] + (H)r[v][i] : (H)x[v][i];
+                ss = fma((double)h[v][i], (double)h[v][i], ss);
+            }
+        if (a.h) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                const int c = column<VW, TPR, VPT>(t, v);
+                float o[VW];
+#pragma unroll
+                for (int i = 0; i < VW; ++i)
+                    o[i] = (float)h[v][i];
+                if (c < a.dim)
+                    store_vec<T, VW>(static_cast<T *>(a.h) + row * a.ld_h + c, o);
+            }
+        }
+        ss = row_sum<double, TPR>(ss, mask, sums);
+        const double rstd64 = 1.0 / sqrt(ss / a.dim + a.eps);
+        const H rstd = (H)rstd64;
+        if (t == 0)
+            a.rstd[row] = (float)rstd64;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                h[v][i] = h[v][i] * rstd * (H)w[v][i];  // y from here on
+                if (a.relu && h[v][i] < (H)0)
+                    h[v][i] = (H)0;
+            }
+        if (a.y) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                const int c = column<VW, TPR, VPT>(t, v);
+                float o[VW];
+#pragma unroll
+                for (int i = 0; i < VW; ++i)
+                    o[i] = (float)h[v][i];
+                if (c < a.dim)
+                    store_vec<T, VW>(static_cast<T *>(a.y) + row * a.ld_y + c, o);
+            }
+        }
+        if constexpr (EIGHT) {
+            // A block is LB lanes wide and SB vectors deep.
+            constexpr int LB = R::LANES * VW >= EIGHT_BLOCK ? EIGHT_BLOCK / VW : R::LANES;
+            constexpr int DEEP = EIGHT_BLOCK / (LB * VW), SB = DEEP < VPT ? DEEP : VPT;
+            static_assert(VPT % SB == 0, "a block spans warps");
+            int8_t *q = a.q + row * a.pitch;
+#pragma unroll
+            for (int v0 = 0; v0 < VPT; v0 += SB) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int v = v0; v < v0 + SB; ++v)
+#pragma unroll
+                    for (int i = 0; i < VW; ++i)
+                        top = max(top, __float_as_uint((float)h[v][i]) & 0x7fffffffu);
+#pragma unroll
+                for (int d = LB / 2; d > 0; d >>= 1)
+                    top = max(top, __shfl_xor_sync(mask, top, d));
+                float scale, up;
+                eight_scale(top, scale, up);
+                const int first = column<VW, TPR, VPT>(t, v0);
+                if (first % EIGHT_BLOCK == 0 && first < a.dim)
+                    a.scales[row * a.blocks + first / EIGHT_BLOCK] = scale;
+#pragma unroll
+                for (int v = v0; v < v0 + SB; ++v) {
+                    const int c = column<VW, TPR, VPT>(t, v);
+                    uint32_t b[VW];
+#pragma unroll
+                    for (int i = 0; i < VW; ++i)
+                        b[i] = eight_round((double)h[v][i], (double)up);
+                    if (c < a.pitch) {  // columns between dim and the pitch hold zeros
+                        if constexpr (VW == 8)
+                            *reinterpret_cast<uint2 *>(q + c) =
+                                make_uint2(pack_bytes(b[0], b[1], b[2], b[3]), pack_bytes(b[4], b[5], b[6], b[7]));
+                        else if constexpr (VW == 4)
+                            *reinterpret_cast<uint32_t *>(q + c) = pack_bytes(b[0], b[1], b[2], b[3]);
+                        else
+                            q[c] = (int8_t)b[0];
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Rows of any width: a CTA per row, two passes.
+template <typename T, bool EIGHT>
+__global__ void __launch_bounds__(1024) norm_wide_kernel(const NormArgs a)
+{
+    using H = typename std::conditional<EIGHT, double, float>::type;
+    __shared__ double sums[32];
+    const T *w = static_cast<const T *>(a.w);
+    for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+        const T *x = static_cast<const T *>(a.x) + row * a.ld_x;
+        const T *r = a.r ? static_cast<const T *>(a.r) + row * a.ld_r : nullptr;
+        double ss = 0;
+        for (int c = threadIdx.x; c < a.dim; c += 1024) {
+            const H h = r ? (H)to_float(x[c]) + (H)to_float(r[c]) : (H)to_float(x[c]);
+            ss = fma((double)h, (double)h, ss);
+        }
+        ss = row_sum<double, 1024>(ss, PSPMM_FULL_MASK, sums);
+        const double rstd64 = 1.0 / sqrt(ss / a.dim + a.eps);
+        const H rstd = (H)rstd64;
+        if (threadIdx.x == 0)
+            a.rstd[row] = (float)rstd64;
+        // A warp takes 128 neighbouring columns at a time, a lane four of them.
+        for (int c0 = threadIdx.x * 4; c0 < (a.dim + EIGHT_BLOCK - 1) / EIGHT_BLOCK * EIGHT_BLOCK; c0 += 4096) {
+            H y[4];
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = c0 + i;
+                y[i] = (H)0;
+                if (c < a.dim) {
+                    const H h = r ? (H)to_float(x[c]) + (H)to_float(r[c]) : (H)to_float(x[c]);
+                    y[i] = h * rstd * (H)to_float(w[c]);
+                    if (a.relu && y[i] < (H)0)
+                        y[i] = (H)0;
+                    if (a.h)
+                        static_cast<T *>(a.h)[row * a.ld_h + c] = from_float<T>((float)h);
+                    if (a.y)
+                        static_cast<T *>(a.y)[row * a.ld_y + c] = from_float<T>((float)y[i]);
+                }
+                top = max(top, __float_as_uint((float)y[i]) & 0x7fffffffu);
+            }
+            if constexpr (EIGHT) {
+                top = __reduce_max_sync(PSPMM_FULL_MASK, top);
+                float scale, up;
+                eight_scale(top, scale, up);
+                if (threadIdx.x % 32 == 0)
+                    a.scales[row * a.blocks + c0 / EIGHT_BLOCK] = scale;
+                uint32_t b[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    b[i] = eight_round((double)y[i], (double)up);
+                if (c0 < a.pitch)
+                    *reinterpret_cast<uint32_t *>(a.q + row * a.pitch + c0) = pack_bytes(b[0], b[1], b[2], b[3]);
+            }
+        }
+    }
+}
+
+template <typename T, int VW, int TPR, int VPT>
+__global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_backward_kernel(const NormBackArgs a)
+{
+    using R = Rows<TPR>;
+    extern __shared__ float warps_dw[];  // [warps][dim] where several rows share a CTA
+    __shared__ float sums[R::THREADS / 32];
+    const int t = threadIdx.x % TPR;
+    const uint32_t mask = group_mask(R::LANES);
+    float w[VPT][VW], dw[VPT][VW] = {};
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        const int c = column<VW, TPR, VPT>(t, v);
+        load_some<T, VW>(w[v], static_cast<const T *>(a.w) + c, c < a.dim);
+    }
+    for (int64_t row = (int64_t)blockIdx.x * R::PER_CTA + threadIdx.x / TPR; row < a.n; row += (int64_t)gridDim.x * R::PER_CTA) {
+        float n[VPT][VW], g[VPT][VW], dh[VPT][VW];
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int c = column<VW, TPR, VPT>(t, v);
+            load_some<T, VW>(n[v], static_cast<const T *>(a.h) + row * a.ld_h + c, c < a.dim);
+            load_some<T, VW>(g[v], static_cast<const T *>(a.dy) + row * a.ld_dy + c, c < a.dim);
+        }
+        if (a.dh) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                const int c = column<VW, TPR, VPT>(t, v);
+                load_some<T, VW>(dh[v], static_cast<const T *>(a.dh) + row * a.ld_dh + c, c < a.dim);
+            }
+        }
+        const float rstd = a.rstd[row];
+        float s = 0;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                n[v][i] *= rstd;
+                if (a.relu && !(n[v][i] * w[v][i] > 0.f))
+                    g[v][i] = 0.f;
+                dw[v][i] = fmaf(g[v][i], n[v][i], dw[v][i]);
+                g[v][i] *= w[v][i];
+                s = fmaf(g[v][i], n[v][i], s);
+            }
+        s = row_sum<float, TPR>(s, mask, sums) / a.dim;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int c = column<VW, TPR, VPT>(t, v);
+            float o[VW];
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                o[i] = (g[v][i] - n[v][i] * s) * rstd;
+                if (a.dh)
+                    o[i] += dh[v][i];
+            }
+            if (c < a.dim)
+                store_vec<T, VW>(static_cast<T *>(a.dx) + row * a.ld_dx + c, o);
+        }
+    }
+    float *part = a.part + (int64_t)blockIdx.x * a.dim;
+    if constexpr (TPR > 32) {
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int c = column<VW, TPR, VPT>(t, v);
+#pragma unroll
+            for (int i = 0; i < VW; ++i)
+                if (c < a.dim)
+                    part[c + i] = dw[v][i];
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+            for (int i = 0; i < VW; ++i)
+#pragma unroll
+                for (int d = 16; d >= TPR; d >>= 1)
+                    dw[v][i] += __shfl_xor_sync(PSPMM_FULL_MASK, dw[v][i], d);
+        if (threadIdx.x % 32 < TPR) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                const int c = column<VW, TPR, VPT>(t, v);
+#pragma unroll
+                for (int i = 0; i < VW; ++i)
+                    if (c < a.dim)
+                        warps_dw[threadIdx.x / 32 * a.dim + c + i] = dw[v][i];
+            }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.dim; c += R::THREADS) {
+            float s = 0;
+#pragma unroll
+            for (int i = 0; i < R::THREADS / 32; ++i)
+                s += warps_dw[i * a.dim + c];
+            part[c] = s;
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_wide_backward_kernel(const NormBackArgs a)
+{
+    __shared__ float sums[32];
+    const T *w = static_cast<const T *>(a.w);
+    float *part = a.part + (int64_t)blockIdx.x * a.dim;
+    for (int c = threadIdx.x; c < a.dim; c += 1024)
+        part[c] = 0.f;
+    for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+        const T *hp = static_cast<const T *>(a.h) + row * a.ld_h, *dy = static_cast<const T *>(a.dy) + row * a.ld_dy;
+        const float rstd = a.rstd[row];
+        float s = 0;
+        for (int c = threadIdx.x; c < a.dim; c += 1024) {
+            const float n = to_float(hp[c]) * rstd;
+            float g = to_float(dy[c]);
+            if (a.relu && !(n * to_float(w[c]) > 0.f))
+                g = 0.f;
+            part[c] = fmaf(g, n, part[c]);  // (a thread meets its own columns only)
+            s = fmaf(g * to_float(w[c]), n, s);
+        }
+        s = row_sum<float, 1024>(s, PSPMM_FULL_MASK, sums) / a.dim;
+        for (int c = threadIdx.x; c < a.dim; c += 1024) {
+            const float n = to_float(hp[c]) * rstd;
+            float g = to_float(dy[c]) * to_float(w[c]);
+            if (a.relu && !(n * to_float(w[c]) > 0.f))
+                g = 0.f;
+            float o = (g - n * s) * rstd;
+            if (a.dh)
+                o += to_float(static_cast<const T *>(a.dh)[row * a.ld_dh + c]);
+            static_cast<T *>(a.dx)[row * a.ld_dx + c] = from_float<T>(o);
+        }
+    }
+}
+
+// dw = sum of the CTAs' parts, in a fixed order: a CTA takes 32 neighbouring columns, its warps the parts in turn.
+__global__ void __launch_bounds__(1024) norm_weight_kernel(const WeightArgs a)
+{
+    __shared__ float sums[32][33];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int c = blockIdx.x * 32 + lane;
+    pdl_wait();
+    float s = 0.f;
+    if (c < a.dim)
+        for (int p = warp; p < a.parts; p += 32)
+            s += a.part[(int64_t)p * a.dim + c];
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && c < a.dim) {
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            s += sums[i][lane];
+        if (a.dtype == PSPMM_F32)
+            static_cast<float *>(a.dw)[c] = s;
+        else if (a.dtype == PSPMM_BF16)
+            static_cast<bf16 *>(a.dw)[c] = from_float<bf16>(s);
+        else
+            static_cast<f16 *>(a.dw)[c] = from_float<f16>(s);
+    }
+}
+
+// CTAs of a launch: as many as find a place, or as there are rows for.
+template <typename K> unsigned resident_grid(K kern, int threads, size_t smem, int64_t ctas)
+{
+    if (ctas <= pspmm_sm_count())
+        return (unsigned)ctas;
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm < 1)
+        per_sm = 1;
+    const int64_t most = (int64_t)per_sm * pspmm_sm_count();
+    return (unsigned)(ctas < most ? ctas : most);
+}
+
+template <typename T, int VW, int TPR, int VPT> cudaError_t launch_forward(const NormArgs &a, cudaStream_t st)
+{
+    using R = Rows<TPR>;
+    const int64_t ctas = (a.n + R::PER_CTA - 1) / R::PER_CTA;
+    if (a.q) {
+        auto kern = norm_kernel<T, VW, TPR, VPT, true>;
+        kern<<<resident_grid(kern, R::THREADS, 0, ctas), R::THREADS, 0, st>>>(a);
+    } else {
+        auto kern = norm_kernel<T, VW, TPR, VPT, false>;
+        kern<<<resident_grid(kern, R::THREADS, 0, ctas), R::THREADS, 0, st>>>(a);
+    }
+    return cudaGetLastError();
+}
+
+// Parts of dw: at most this many, so that scratch can be sized without a look at the kernels.
+constexpr int PARTS_PER_SM = 8;
+int64_t most_parts(int64_t n) { return n < (int64_t)PARTS_PER_SM * pspmm_sm_count() ? n : (int64_t)PARTS_PER_SM * pspmm_sm_count(); }
+
+template <typename T, int VW, int TPR, int VPT> cudaError_t launch_backward(const NormBackArgs &a, unsigned &parts, cudaStream_t st)
+{
+    using R = Rows<TPR>;
+    auto kern = norm_backward_kernel<T, VW, TPR, VPT>;
+    const size_t smem = TPR > 32 ? 0 : (size_t)(R::THREADS / 32) * a.dim * 4;  // (at most 8 x 512 columns: 16 KB)
+    int64_t ctas = (a.n + R::PER_CTA - 1) / R::PER_CTA;
+    ctas = ctas < most_parts(a.n) ? ctas : most_parts(a.n);
+    parts = resident_grid(kern, R::THREADS, smem, ctas);
+    kern<<<parts, R::THREADS, smem, st>>>(a);
+    return cudaGetLastError();
+}
+
+struct Forward {
+    const NormArgs &a;
+    cudaStream_t st;
+    template <typename T, int VW, int TPR, int VPT> cudaError_t run() { return launch_forward<T, VW, TPR, VPT>(a, st); }
+};
+struct Backward {
+    const NormBackArgs &a;
+    unsigned &parts;
+    cudaStream_t st;
+    template <typename T, int VW, int TPR, int VPT> cudaError_t run() { return launch_backward<T, VW, TPR, VPT>(a, parts, st); }
+};
+
+// Fewest threads that hold a row in 16 values each (8 where they come singly, and less in narrow rows); false beyond 8,192 columns.
+// (More would spill beside 64-bit copies, fewer leave too few loads in flight.)
+template <typename T, int VW, typename L> bool by_width(int dim, L l, cudaError_t &e)
+{
+    const int nv = (dim + VW - 1) / VW;
+    if constexpr (VW == 1) {
+        if (nv <= 32) e = l.template run<T, 1, 8, 4>();
+        else if (nv <= 128) e = l.template run<T, 1, 32, 4>();
+        else if (nv <= 256) e = l.template run<T, 1, 32, 8>();
+        else if (nv <= 1024) e = l.template run<T, 1, 128, 8>();
+        else if (nv <= 4096) e = l.template run<T, 1, 512, 8>();
+        else if (nv <= 8192) e = l.template run<T, 1, 1024, 8>();
+        else return false;
+    } else if constexpr (VW == 8) {
+        if (nv <= 8) e = l.template run<T, 8, 8, 1>();
+        else if (nv <= 16) e = l.template run<T, 8, 8, 2>();
+        else if (nv <= 32) e = l.template run<T, 8, 16, 2>();
+        else if (nv <= 64) e = l.template run<T, 8, 32, 2>();
+        else if (nv <= 128) e = l.template run<T, 8, 64, 2>();
+        else if (nv <= 256) e = l.template run<T, 8, 128, 2>();
+        else if (nv <= 512) e = l.template run<T, 8, 256, 2>();
+        else if (nv <= 1024) e = l.template run<T, 8, 512, 2>();
+        else return false;
+    } else {
+        if (nv <= 8) e = l.template run<T, VW, 8, 1>();
+        else if (nv <= 16) e = l.template run<T, VW, 8, 2>();
+        else if (nv <= 32) e = l.template run<T, VW, 8, 4>();
+        else if (nv <= 64) e = l.template run<T, VW, 16, 4>();
+        else if (nv <= 128) e = l.template run<T, VW, 32, 4>();
+        else if (nv <= 256) e = l.template run<T, VW, 64, 4>();
+        else if (nv <= 512) e = l.template run<T, VW, 128, 4>();
+        else if (nv <= 1024) e = l.template run<T, VW, 256, 4>();
+        else if (nv <= 2048) e = l.template run<T, VW, 512, 4>();
+        else return false;
+    }
+    return true;
+}
+
+template <typename T> cudaError_t forward_typed(const NormArgs &a, cudaStream_t st)
+{
+    constexpr int B = sizeof(T), WIDE = 16 / B;
+    auto aligned = [&](int bytes) {
+        return a.dim * B % bytes == 0 && rows_aligned(a.x, a.ld_x, B, bytes) && rows_aligned(a.r, a.ld_r, B, bytes) &&
+               rows_aligned(a.h, a.ld_h, B, bytes) && rows_aligned(a.y, a.ld_y, B, bytes) && rows_aligned(a.w, 0, B, bytes);
+    };
+    cudaError_t e = cudaSuccess;
+    const Forward l = {a, st};
+    if (aligned(16) && by_width<T, WIDE>(a.dim, l, e))
+        return e;
+    if constexpr (B == 2)
+        if (aligned(8) && by_width<T, 4>(a.dim, l, e))
+            return e;
+    if (by_width<T, 1>(a.dim, l, e))
+        return e;
+    const unsigned grid = (unsigned)(a.n < 2 * pspmm_sm_count() ? a.n : 2 * pspmm_sm_count());
+    if (a.q)
+        norm_wide_kernel<T, true><<<grid, 1024, 0, st>>>(a);
+    else
+        norm_wide_kernel<T, false><<<grid, 1024, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T> cudaError_t backward_typed(const NormBackArgs &a, unsigned &parts, cudaStream_t st)
+{
+    constexpr int B = sizeof(T), WIDE = 16 / B;
+    auto aligned = [&](int bytes) {
+        return a.dim * B % bytes == 0 && rows_aligned(a.dy, a.ld_dy, B, bytes) && rows_aligned(a.h, a.ld_h, B, bytes) &&
+               rows_aligned(a.dh, a.ld_dh, B, bytes) && rows_aligned(a.dx, a.ld_dx, B, bytes) && rows_aligned(a.w, 0, B, bytes);
+    };
+    cudaError_t e = cudaSuccess;
+    const Backward l = {a, parts, st};
+    if (aligned(16) && by_width<T, WIDE>(a.dim, l, e))
+        return e;
+    if constexpr (B == 2)
+        if (aligned(8) && by_width<T, 4>(a.dim, l, e))
+            return e;
+    if (by_width<T, 1>(a.dim, l, e))
+        return e;
+    const int64_t most = most_parts(a.n);
+    parts = (unsigned)(most < 2 * pspmm_sm_count() ? most : 2 * pspmm_sm_count());
+    norm_wide_backward_kernel<T><<<parts, 1024, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+bool bad(const void *p, int64_t ld, int32_t dim, int bytes) { return ld < dim || (uintptr_t)p % bytes != 0; }
+
+}  // namespace
+
+extern "C" int pspmm_rms_norm(const void *x, int64_t ld_x, const void *residual, int64_t ld_residual, const void *weight,
+                              int32_t dtype, int64_t n, int32_t dim, double eps, int32_t relu, void *h, int64_t ld_h, void *y,
+                              int64_t ld_y, float *rstd, int8_t *q, int64_t pitch, float *scales, void *stream)
+{
+    if (!dtype_ok(dtype) || n < 0 || dim < 1 || !(eps >= 0) || ld_x < dim || (residual && ld_residual < dim) ||
+        (h && ld_h < dim) || (y && ld_y < dim) || (q && (pitch < dim || pitch % 16 != 0)) || !q != !scales)
+        return PSPMM_E_ARG;
+    if (n == 0)
+        return PSPMM_OK;
+    const int B = elem_bytes(dtype);
+    if (!x || !weight || !rstd || bad(x, ld_x, 0, B) || bad(residual, 0, 0, B) || bad(weight, 0, 0, B) || bad(h, 0, 0, B) ||
+        bad(y, 0, 0, B) || (uintptr_t)rstd % 4 != 0 || (uintptr_t)q % 16 != 0 || (uintptr_t)scales % 4 != 0)
+        return PSPMM_E_ARG;
+    if (pitch > INT32_MAX - 8192 || dim > INT32_MAX - 8192)
+        return PSPMM_E_RANGE;
+    const NormArgs a = {x, residual, weight, h, y, rstd, q, scales, n, ld_x, ld_residual, ld_h, ld_y, eps, dim,
+                        (int32_t)pitch, (dim + EIGHT_BLOCK - 1) / EIGHT_BLOCK, relu};
+    cudaStream_t st = (cudaStream_t)stream;
+    PSPMM_CUDA_TRY(dtype == PSPMM_F32    ? forward_typed<float>(a, st)
+                   : dtype == PSPMM_BF16 ? forward_typed<bf16>(a, st)
+                                         : forward_typed<f16>(a, st));
+    return PSPMM_OK;
+}
+
+extern "C" int pspmm_rms_norm_backward_scratch_bytes(int64_t n, int32_t dim, size_t *bytes)
+{
+    if (n < 0 || dim < 1 || !bytes)
+        return PSPMM_E_ARG;
+    *bytes = (size_t)most_parts(n) * (size_t)dim * 4;
+    return PSPMM_OK;
+}
+
+extern "C" int pspmm_rms_norm_backward(const void *dy, int64_t ld_dy, const void *h, int64_t ld_h, const float *rstd,
+                                       const void *weight, const void *dh, int64_t ld_dh, int32_t dtype, int64_t n, int32_t dim,
+                                       int32_t relu, void *dx, int64_t ld_dx, void *dweight, void *scratch, size_t scratch_bytes,
+                                       void *stream)
+{
+    if (!dtype_ok(dtype) || n < 0 || dim < 1 || ld_dy < dim || ld_h < dim || (dh && ld_dh < dim) || ld_dx < dim)
+        return PSPMM_E_ARG;
+    const int B = elem_bytes(dtype);
+    if (!dweight || bad(dweight, 0, 0, B))
+        return PSPMM_E_ARG;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (n == 0) {
+        PSPMM_CUDA_TRY(cudaMemsetAsync(dweight, 0, (size_t)dim * B, st));
+        return PSPMM_OK;
+    }
+    if (!dy || !h || !rstd || !weight || !dx || !scratch || bad(dy, 0, 0, B) || bad(h, 0, 0, B) || bad(weight, 0, 0, B) ||
+        bad(dh, 0, 0, B) || bad(dx, 0, 0, B) || (uintptr_t)rstd % 4 != 0 || (uintptr_t)scratch % 4 != 0 ||
+        scratch_bytes < (size_t)most_parts(n) * (size_t)dim * 4)
+        return PSPMM_E_ARG;
+    if (dim > INT32_MAX - 8192)
+        return PSPMM_E_RANGE;
+    const NormBackArgs a = {dy, h, weight, dh, rstd, dx, (float *)scratch, n, ld_dy, ld_h, ld_dh, ld_dx, dim, relu};
+    unsigned parts = 0;
+    PSPMM_CUDA_TRY(dtype == PSPMM_F32    ? backward_typed<float>(a, parts, st)
+                   : dtype == PSPMM_BF16 ? backward_typed<bf16>(a, parts, st)
+                                         : backward_typed<f16>(a, parts, st));
+    const WeightArgs wa = {(const float *)scratch, dweight, (int32_t)parts, dim, dtype};
+    PSPMM_CUDA_TRY(launch_dependent(norm_weight_kernel, dim3((unsigned)((dim + 31) / 32)), 1024, 0, st, wa));
+    return PSPMM_OK;
+}

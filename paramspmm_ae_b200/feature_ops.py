@@ -1,0 +1,246 @@
+"""Operators around the graph layers, over libpspmm's C ABI: embedding lookup and its gradient, the
+root-mean-square norm of a residual stream, and activations held in 8 bits.
+
+They are tensor-level calls like those of ``ops`` (no autograd; ``gnn_conv`` has the layers that train
+with them).  Element types: float32, bfloat16 and float16, sums in 32 bits or more.  2-D operands may be
+row-strided views; every operand of a call lives on one GPU, which need not be the current one, and the
+work goes to that GPU's current stream.  There is no CPU or PyTorch fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from ._lib import check, lib
+from .ops import _ptr, _scratch, _stream
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PSPMM_F32 / _BF16 / _F16
+EIGHT_BLOCK = 128  # columns that share a scale in the 8-bit form
+MAX_DIM = 1 << 24
+
+
+def _gpu_of(*tensors):
+    """The one device of the operands (None among them: left out)."""
+    gpu = None
+    for name, t in tensors:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise RuntimeError("%s must be a tensor" % name)
+        if not t.is_cuda:
+            raise RuntimeError("%s must be a CUDA tensor" % name)
+        if gpu is None:
+            gpu = t.get_device()
+        elif t.get_device() != gpu:
+            raise RuntimeError("%s is on another device than the other operands" % name)
+    return gpu
+
+
+def _elsewhere(gpu):
+    return gpu != torch._C._cuda_getDevice()
+
+
+def _rows(t, name, dtype=None, shape=None):
+    """(rows, columns, leading dimension) of a matrix with unit column stride, or of a contiguous array with more or fewer
+    dimensions taken as rows of its last one."""
+    if t.dtype not in _DTYPES or (dtype is not None and t.dtype is not dtype):
+        raise RuntimeError("%s must have dtype %s, got %s" % (name, dtype or "float32, bfloat16 or float16", t.dtype))
+    if shape is not None and t.shape != shape:
+        raise RuntimeError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    if t.dim() == 0 or t.shape[-1] == 0 or t.shape[-1] > MAX_DIM:
+        raise RuntimeError("%s must have between 1 and %d columns" % (name, MAX_DIM))
+    dim = t.shape[-1]
+    if t.is_contiguous():
+        return t.numel() // dim, dim, dim
+    if t.dim() == 2 and (t.stride(1) == 1 or dim == 1) and t.stride(0) >= dim:
+        return t.shape[0], dim, t.stride(0)
+    raise RuntimeError("%s must be contiguous, or a matrix whose rows are" % name)
+
+
+def _vector(t, name, dim, dtype):
+    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != dim or not t.is_contiguous():
+        raise RuntimeError("%s must be a contiguous %s vector of %d" % (name, dtype, dim))
+
+
+# ----------------------------------------------------------------------------- embedding
+def _ids(ids):
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError("ids must be int32 or int64, got %s" % ids.dtype)
+    if not ids.is_contiguous():
+        raise RuntimeError("ids must be contiguous")
+    return 1 if ids.dtype is torch.int64 else 0
+
+
+def embedding(ids, table, scale=1.0):
+    """``scale * table[ids]``: one row of ``table`` ([rows, dim]) per id, of the table's type, shaped ``ids.shape + (dim,)``.
+
+    An id outside the table gives a row of NaN and sets :func:`embedding_status` (the GPU is not waited for)."""
+    gpu = _gpu_of(("ids", ids), ("table", table))
+    if _elsewhere(gpu):
+        with torch.cuda.device(gpu):
+            return embedding(ids, table, scale)
+    wide = _ids(ids)
+    if table.dim() != 2:
+        raise RuntimeError("table must be 2-dimensional")
+    rows, dim, ld = _rows(table, "table")
+    out = torch.empty(ids.shape + (dim,), dtype=table.dtype, device=table.device)
+    rc = lib().pspmm_embedding(ids.data_ptr(), wide, ids.numel(), table.data_ptr(), _DTYPES[table.dtype], rows, dim, ld, scale,
+                               out.data_ptr(), dim, _stream())
+    if rc:
+        check(rc)
+    return out
+
+
+def embedding_grad(ids, grad, n_rows, scale=1.0, padding_idx=None):
+    """Gradient of :func:`embedding` with respect to its table of ``n_rows`` rows: row t is ``scale`` times the sum of the rows of
+    ``grad`` whose id is t, of the type of ``grad``; ids equal to ``padding_idx`` and ids outside the table add nothing.
+
+    The sums run in the order of the ids' positions (they are sorted first): equal calls give equal bits."""
+    gpu = _gpu_of(("ids", ids), ("grad", grad))
+    if _elsewhere(gpu):
+        with torch.cuda.device(gpu):
+            return embedding_grad(ids, grad, n_rows, scale, padding_idx)
+    wide = _ids(ids)
+    n, dim, ld = _rows(grad, "grad")
+    if n != ids.numel():
+        raise RuntimeError("grad must have one row per id")
+    if n_rows < 0:
+        raise RuntimeError("n_rows must not be negative")
+    if padding_idx is not None and not 0 <= padding_idx < n_rows:
+        raise RuntimeError("padding_idx must be a row of the table")
+    out = torch.empty((n_rows, dim), dtype=grad.dtype, device=grad.device)
+    scratch, need = _scratch("pspmm_embedding_grad_scratch_bytes", (n, dim), grad.device)
+    rc = lib().pspmm_embedding_grad(ids.data_ptr(), wide, n, grad.data_ptr(), _DTYPES[grad.dtype], ld, n_rows, dim, scale,
+                                    -1 if padding_idx is None else padding_idx, out.data_ptr(), dim, _ptr(scratch), need, _stream())
+    if rc:
+        check(rc)
+    return out
+
+
+def embedding_status():
+    """1 once an id outside its table has been met in this process on the current GPU, else 0 (synchronises with the device)."""
+    v = ctypes.c_int32(0)
+    check(lib().pspmm_embedding_status(ctypes.byref(v)))
+    return int(v.value)
+
+
+# ----------------------------------------------------------------------------- rows in 8 bits
+class Rows8:
+    """Rows held in 8 bits: per row and block of 128 columns with largest magnitude a, ``scale = a / 127`` and whole numbers
+    ``q = rint(x * (127 / a))``; ``q * scale`` stands for ``x`` and is off by at most 0.51 scale.  Blocks below 2^-119 are
+    zeros, blocks with an infinity or a NaN come back as NaN.
+
+    ``q``: int8 [n, pitch], rows padded to a multiple of 16 bytes; ``scales``: float32 [n, ceil(dim / 128)]; ``shape`` is that of
+    the array held."""
+
+    __slots__ = ("q", "scales", "dim", "shape")
+
+    def __init__(self, q, scales, dim, shape=None):
+        n = q.shape[0] if q.dim() == 2 else -1
+        if (q.dtype is not torch.int8 or n < 0 or not q.is_contiguous() or q.shape[1] < dim or q.shape[1] % 16 or dim < 1
+                or q.data_ptr() % 16):
+            raise RuntimeError("q must be a contiguous, 16-byte aligned int8 matrix of rows padded to a multiple of 16, at least %d"
+                               % dim)
+        if (scales.dtype is not torch.float32 or not scales.is_contiguous()
+                or scales.shape != (n, (dim + EIGHT_BLOCK - 1) // EIGHT_BLOCK)):
+            raise RuntimeError("scales must be a contiguous float32 matrix of a scale per row and block of %d columns" % EIGHT_BLOCK)
+        if q.get_device() != scales.get_device():
+            raise RuntimeError("scales is on another device than q")
+        self.q, self.scales, self.dim = q, scales, dim
+        self.shape = torch.Size((n, dim)) if shape is None else torch.Size(shape)
+        if self.shape[-1] != dim or self.shape.numel() != n * dim:
+            raise RuntimeError("shape must be that of %d rows of %d" % (n, dim))
+
+    def dequantize(self, dtype=torch.float32):
+        """The values that the whole numbers stand for."""
+        gpu = _gpu_of(("q", self.q), ("scales", self.scales))
+        if _elsewhere(gpu):
+            with torch.cuda.device(gpu):
+                return self.dequantize(dtype)
+        if dtype not in _DTYPES:
+            raise RuntimeError("dtype must be float32, bfloat16 or float16, got %s" % dtype)
+        out = torch.empty(self.shape, dtype=dtype, device=self.q.device)
+        rc = lib().pspmm_dequantize_rows(self.q.data_ptr(), self.q.shape[1], self.scales.data_ptr(), _DTYPES[dtype], out.data_ptr(),
+                                         self.dim, self.q.shape[0], self.dim, _stream())
+        if rc:
+            check(rc)
+        return out
+
+
+def _empty_rows8(n, dim, device):
+    return (torch.empty((n, dim + -dim % 16), dtype=torch.int8, device=device),
+            torch.empty((n, (dim + EIGHT_BLOCK - 1) // EIGHT_BLOCK), dtype=torch.float32, device=device))
+
+
+def quantize_rows(x):
+    """``x`` in 8 bits (:class:`Rows8`), a scale per row and 128 columns."""
+    gpu = _gpu_of(("x", x))
+    if _elsewhere(gpu):
+        with torch.cuda.device(gpu):
+            return quantize_rows(x)
+    n, dim, ld = _rows(x, "x")
+    q, scales = _empty_rows8(n, dim, x.device)
+    rc = lib().pspmm_quantize_rows(x.data_ptr(), _DTYPES[x.dtype], ld, n, dim, q.data_ptr(), q.shape[1], scales.data_ptr(), _stream())
+    if rc:
+        check(rc)
+    return Rows8(q, scales, dim, x.shape)
+
+
+# ----------------------------------------------------------------------------- norm
+def rms_norm(x, weight, residual=None, eps=1e-6, relu=False, values=True, eight_bit=False):
+    """Root-mean-square norm of ``h = x + residual`` over the last dimension: ``y = h * rstd * weight`` with
+    ``rstd = (mean(h^2) + eps)^-1/2``, negative ``y`` set to 0 with ``relu``.
+
+    Returns ``(y, h, rstd, kept)``: ``h`` is the residual stream (``x`` itself without a ``residual``), ``rstd`` (float32, one per
+    row) what :func:`rms_norm_backward` needs, ``kept`` the :class:`Rows8` of ``y`` with ``eight_bit`` (else None), made in the
+    same pass.  ``values=False`` leaves ``y`` out (None) for a consumer of the 8 bits alone."""
+    gpu = _gpu_of(("x", x), ("weight", weight), ("residual", residual))
+    if _elsewhere(gpu):
+        with torch.cuda.device(gpu):
+            return rms_norm(x, weight, residual, eps, relu, values, eight_bit)
+    n, dim, ld = _rows(x, "x")
+    _vector(weight, "weight", dim, x.dtype)
+    if not eps >= 0:
+        raise RuntimeError("eps must not be negative")
+    if not values and not eight_bit:
+        raise RuntimeError("nothing is asked for: neither values nor the 8-bit form")
+    h, ld_r = x, 0
+    if residual is not None:
+        ld_r = _rows(residual, "residual", x.dtype, x.shape)[2]
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if values else None
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    q = scales = None
+    if eight_bit:
+        q, scales = _empty_rows8(n, dim, x.device)
+    rc = lib().pspmm_rms_norm(x.data_ptr(), ld, _ptr(residual), ld_r, weight.data_ptr(), _DTYPES[x.dtype], n, dim, eps,
+                              1 if relu else 0, None if residual is None else h.data_ptr(), dim, _ptr(y), dim, rstd.data_ptr(),
+                              _ptr(q), q.shape[1] if eight_bit else 0, _ptr(scales), _stream())
+    if rc:
+        check(rc)
+    return y, h, rstd, Rows8(q, scales, dim, x.shape) if eight_bit else None
+
+
+def rms_norm_backward(dy, h, rstd, weight, dh=None, relu=False):
+    """Gradients ``(dx, dweight)`` of :func:`rms_norm` from ``dy`` and, where the residual stream goes on, the gradient ``dh`` that
+    reaches ``h`` itself; ``dx`` is the gradient of ``x`` and of ``residual`` alike."""
+    gpu = _gpu_of(("dy", dy), ("h", h), ("rstd", rstd), ("weight", weight), ("dh", dh))
+    if _elsewhere(gpu):
+        with torch.cuda.device(gpu):
+            return rms_norm_backward(dy, h, rstd, weight, dh, relu)
+    n, dim, ld_h = _rows(h, "h")
+    ld_dy = _rows(dy, "dy", h.dtype, h.shape)[2]
+    ld_dh = _rows(dh, "dh", h.dtype, h.shape)[2] if dh is not None else 0
+    _vector(weight, "weight", dim, h.dtype)
+    if rstd.dtype is not torch.float32 or rstd.shape != h.shape[:-1] or not rstd.is_contiguous():
+        raise RuntimeError("rstd must be contiguous float32, one per row")
+    dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    dw = torch.empty_like(weight)
+    scratch, need = _scratch("pspmm_rms_norm_backward_scratch_bytes", (n, dim), h.device)
+    rc = lib().pspmm_rms_norm_backward(dy.data_ptr(), ld_dy, h.data_ptr(), ld_h, rstd.data_ptr(), weight.data_ptr(), _ptr(dh), ld_dh,
+                                       _DTYPES[h.dtype], n, dim, 1 if relu else 0, dx.data_ptr(), dim, dw.data_ptr(), _ptr(scratch),
+                                       need, _stream())
+    if rc:
+        check(rc)
+    return dx, dw
