@@ -405,6 +405,23 @@ PSPMM_API int pspmm_dequantize_rows(const int8_t *q, int64_t pitch, const float 
                                     int64_t n, int32_t dim, void *stream);
 
 /*
+ * C[dim, cols] = X^T G, fp32, where X[n, dim] is held in the 8-bit form (q, scales) and G[n, cols] has element type dtype: the weight
+ * gradient of a layer that kept its input in 8 bits.  On the tensor cores with fp32 accuracy: q is exact in bf16, scale * G (rounded
+ * to fp32) is cut into three bf16 parts whose sum it is.  Any size and alignment of G.  Scratch:
+ * pspmm_rows8_mm_t_scratch_bytes(n, dim, cols) bytes, 16-byte aligned.  n == 0 gives zeros.  Waits inside the kernel are bounded (two
+ * seconds): when one runs out, what was not computed of C becomes NaN and pspmm_rows8_mm_status returns 1 from then on in this
+ * process (it synchronises).  pspmm_rows8_mm_t_stalled is for tests of that path, as pspmm_dense_mm_stalled.
+ */
+PSPMM_API int pspmm_rows8_mm_t_scratch_bytes(int64_t n, int32_t dim, int32_t cols, size_t *bytes);
+PSPMM_API int pspmm_rows8_mm_t(const int8_t *q, int64_t pitch, const float *scales, int64_t n, int32_t dim, const void *G,
+                               int32_t dtype, int64_t ldG, int32_t cols, float *C, int64_t ldC, void *scratch,
+                               size_t scratch_bytes, void *stream);
+PSPMM_API int pspmm_rows8_mm_t_stalled(const int8_t *q, int64_t pitch, const float *scales, int64_t n, int32_t dim, const void *G,
+                               int32_t dtype, int64_t ldG, int32_t cols, float *C, int64_t ldC, void *scratch,
+                               size_t scratch_bytes, void *stream);
+PSPMM_API int pspmm_rows8_mm_status(int32_t *status);
+
+/*
  * Root-mean-square norm with the residual's addition:
  *     h = x + residual,   rstd = (mean(h^2) + eps)^-1/2,   y = h * rstd * weight   (relu != 0: negative y become 0)
  * residual may be NULL (h = x).  h and y may each be NULL: not wanted.  rstd[n] is always written.  q / scales (both or

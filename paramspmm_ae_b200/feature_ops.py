@@ -187,6 +187,38 @@ def quantize_rows(x):
     return Rows8(q, scales, dim, x.shape)
 
 
+def rows8_mm_t(rows, G, out=None):
+    """``X^T @ G`` in float32, [dim, cols], from the 8-bit form of X ([n, dim], a :class:`Rows8`) and ``G`` ([n, cols]): the weight
+    gradient of a layer that kept its input in 8 bits, on the tensor cores with float32 accuracy."""
+    if not isinstance(rows, Rows8):
+        raise RuntimeError("rows must be a Rows8")
+    gpu = _gpu_of(("q", rows.q), ("scales", rows.scales), ("G", G), ("out", out))
+    if _elsewhere(gpu):
+        with torch.cuda.device(gpu):
+            return rows8_mm_t(rows, G, out)
+    n, cols, ld = _rows(G, "G")
+    if n != rows.q.shape[0]:
+        raise RuntimeError("G must have one row per row held, %d, got %d" % (rows.q.shape[0], n))
+    if out is None:
+        out = torch.empty((rows.dim, cols), dtype=torch.float32, device=G.device)
+    elif (out.dtype is not torch.float32 or out.shape != (rows.dim, cols) or out.stride(1) != 1 or out.stride(0) < cols):
+        raise RuntimeError("out must be a float32 matrix of %d rows of %d with unit column stride" % (rows.dim, cols))
+    scratch, need = _scratch("pspmm_rows8_mm_t_scratch_bytes", (n, rows.dim, cols), G.device)
+    rc = lib().pspmm_rows8_mm_t(rows.q.data_ptr(), rows.q.shape[1], rows.scales.data_ptr(), n, rows.dim, G.data_ptr(),
+                                _DTYPES[G.dtype], ld, cols, out.data_ptr(), out.stride(0), _ptr(scratch), need, _stream())
+    if rc:
+        check(rc)
+    return out
+
+
+def rows8_mm_status():
+    """1 once a bounded wait of :func:`rows8_mm_t` has run out in this process on the current GPU, else 0 (synchronises with the
+    device).  What was not computed of the result is NaN then."""
+    v = ctypes.c_int32(0)
+    check(lib().pspmm_rows8_mm_status(ctypes.byref(v)))
+    return int(v.value)
+
+
 # ----------------------------------------------------------------------------- norm
 def rms_norm(x, weight, residual=None, eps=1e-6, relu=False, values=True, eight_bit=False):
     """Root-mean-square norm of ``h = x + residual`` over the last dimension: ``y = h * rstd * weight`` with

@@ -150,3 +150,24 @@ def test_operands_on_two_gpus_are_refused():
                  lambda: fo.embedding_grad(ids, a, 5), lambda: fo.rms_norm_backward(a, b, w, w)):
         with pytest.raises(RuntimeError, match="another device"):
             call()
+
+
+def test_rows8_product_entry_point_refuses(pspmm_lib):
+    from paramspmm_ae_b200 import _lib
+    need = ctypes.c_size_t(0)
+    assert pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(100000, 64, 16, ctypes.byref(need)) == 0 and need.value > 0
+    size = need.value
+    assert pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(0, 64, 16, ctypes.byref(need)) == 0 and need.value == 0
+    _arg(pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(-1, 64, 16, ctypes.byref(need)))
+    _arg(pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(1, 64, 16, None))
+
+    def mm(q=ONE, pitch=64, s=ONE, n=100000, dim=64, G=ONE, t=0, ld=16, cols=16, C=ONE, ldc=16, scratch=ONE, size=size):
+        return pspmm_lib.pspmm_rows8_mm_t(q, pitch, s, n, dim, G, t, ld, cols, C, ldc, scratch, size, NULL)
+
+    for bad in (dict(q=NULL), dict(s=NULL), dict(G=NULL), dict(C=NULL), dict(scratch=NULL), dict(size=size - 1), dict(pitch=63),
+                dict(pitch=72), dict(pitch=48), dict(n=-1), dict(dim=0), dict(t=3), dict(ld=15), dict(ldc=15), dict(cols=-1),
+                dict(q=ctypes.c_void_p(4104)), dict(G=ctypes.c_void_p(4098)), dict(scratch=ctypes.c_void_p(4104))):
+        _arg(mm(**bad))
+    assert mm(n=1 << 50) == _lib.PSPMM_E_RANGE
+    assert mm(cols=1 << 21, ld=1 << 21, ldc=1 << 21) == _lib.PSPMM_E_RANGE
+    assert mm(cols=0, C=NULL, G=NULL) == _lib.PSPMM_OK
