@@ -7,12 +7,10 @@
 // 32 lanes (several rows per warp) with up to 16 values each, a CTA of 64 to 1,024 threads beyond that, and two passes over a row
 // wider than 8,192 columns.
 //
-// Numbers: the sum x + r is formed in 32 bits and the squares are added in 64 (which costs nothing here: about six 64-bit
-// operations per value where the memory system leaves time for twenty).  Where y leaves in 8 bits, h, rstd and y are in 64 bits throughout,
-// because next to a half the last bit of a 32-bit y decides which whole number it becomes.  rstd is kept in 32 bits for the backward,
-// whose sums are in 32 bits.
-#include <type_traits>
-
+// Numbers: the squares are added in 64 bits, which costs nothing here (the 64-bit units run at half the 32-bit rate and the memory
+// system leaves them idle).  y in 8 bits is taken from h, rstd and y in 64 bits throughout, because next to a half the last bit of
+// a 32-bit y decides which whole number it becomes; y itself is the 32-bit one with and without it.  rstd is kept in 32 bits for the
+// backward, whose sums are in 32 bits.
 #include "feature_types.cuh"
 
 namespace {
@@ -104,7 +102,6 @@ template <typename T, int VW, int TPR, int VPT, bool EIGHT>
 __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs a)
 {
     using R = Rows<TPR>;
-    using H = typename std::conditional<EIGHT, double, float>::type;
     __shared__ double sums[R::THREADS / 32];
     const int t = threadIdx.x % TPR;
     const uint32_t mask = group_mask(R::LANES);
@@ -128,50 +125,43 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs
                 load_some<T, VW>(r[v], static_cast<const T *>(a.r) + row * a.ld_r + c, c < a.dim);
             }
         }
-        H h[VPT][VW];
-        double ss = 0;
+        double ss = 0, ss64 = 0;
+        float h[VPT][VW];
 #pragma unroll
         for (int v = 0; v < VPT; ++v)
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
-                h[v][i] = a.r ? (H)x[v][i] + (H)r[v][i] : (H)x[v][i];
+                h[v][i] = a.r ? x[v][i] + r[v][i] : x[v][i];
                 ss = fma((double)h[v][i], (double)h[v][i], ss);
+                if constexpr (EIGHT) {
+                    const double h64 = a.r ? (double)x[v][i] + (double)r[v][i] : (double)x[v][i];
+                    ss64 = fma(h64, h64, ss64);
+                }
             }
         if (a.h) {
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
                 const int c = column<VW, TPR, VPT>(t, v);
-                float o[VW];
-#pragma unroll
-                for (int i = 0; i < VW; ++i)
-                    o[i] = (float)h[v][i];
                 if (c < a.dim)
-                    store_vec<T, VW>(static_cast<T *>(a.h) + row * a.ld_h + c, o);
+                    store_vec<T, VW>(static_cast<T *>(a.h) + row * a.ld_h + c, h[v]);
             }
         }
         ss = row_sum<double, TPR>(ss, mask, sums);
-        const double rstd64 = 1.0 / sqrt(ss / a.dim + a.eps);
-        const H rstd = (H)rstd64;
+        const float rstd = (float)(1.0 / sqrt(ss / a.dim + a.eps));
         if (t == 0)
-            a.rstd[row] = (float)rstd64;
-#pragma unroll
-        for (int v = 0; v < VPT; ++v)
-#pragma unroll
-            for (int i = 0; i < VW; ++i) {
-                h[v][i] = h[v][i] * rstd * (H)w[v][i];  // y from here on
-                if (a.relu && h[v][i] < (H)0)
-                    h[v][i] = (H)0;
-            }
+            a.rstd[row] = rstd;
         if (a.y) {
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
                 const int c = column<VW, TPR, VPT>(t, v);
-                float o[VW];
 #pragma unroll
-                for (int i = 0; i < VW; ++i)
-                    o[i] = (float)h[v][i];
+                for (int i = 0; i < VW; ++i) {
+                    h[v][i] = h[v][i] * rstd * w[v][i];  // y
+                    if (a.relu && h[v][i] < 0.f)
+                        h[v][i] = 0.f;
+                }
                 if (c < a.dim)
-                    store_vec<T, VW>(static_cast<T *>(a.y) + row * a.ld_y + c, o);
+                    store_vec<T, VW>(static_cast<T *>(a.y) + row * a.ld_y + c, h[v]);
             }
         }
         if constexpr (EIGHT) {
@@ -179,15 +169,24 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs
             constexpr int LB = R::LANES * VW >= EIGHT_BLOCK ? EIGHT_BLOCK / VW : R::LANES;
             constexpr int DEEP = EIGHT_BLOCK / (LB * VW), SB = DEEP < VPT ? DEEP : VPT;
             static_assert(VPT % SB == 0, "a block spans warps");
+            ss64 = row_sum<double, TPR>(ss64, mask, sums);
+            const double rstd64 = 1.0 / sqrt(ss64 / a.dim + a.eps);
             int8_t *q = a.q + row * a.pitch;
 #pragma unroll
             for (int v0 = 0; v0 < VPT; v0 += SB) {
+                double y[SB][VW];
                 uint32_t top = 0;
 #pragma unroll
-                for (int v = v0; v < v0 + SB; ++v)
+                for (int v = 0; v < SB; ++v)
 #pragma unroll
-                    for (int i = 0; i < VW; ++i)
-                        top = max(top, __float_as_uint((float)h[v][i]) & 0x7fffffffu);
+                    for (int i = 0; i < VW; ++i) {
+                        const float xi = x[v0 + v][i];
+                        const double h64 = a.r ? (double)xi + (double)r[v0 + v][i] : (double)xi;
+                        y[v][i] = h64 * rstd64 * (double)w[v0 + v][i];
+                        if (a.relu && y[v][i] < 0.0)
+                            y[v][i] = 0.0;
+                        top = max(top, __float_as_uint((float)y[v][i]) & 0x7fffffffu);
+                    }
 #pragma unroll
                 for (int d = LB / 2; d > 0; d >>= 1)
                     top = max(top, __shfl_xor_sync(mask, top, d));
@@ -197,12 +196,12 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs
                 if (first % EIGHT_BLOCK == 0 && first < a.dim)
                     a.scales[row * a.blocks + first / EIGHT_BLOCK] = scale;
 #pragma unroll
-                for (int v = v0; v < v0 + SB; ++v) {
-                    const int c = column<VW, TPR, VPT>(t, v);
+                for (int v = 0; v < SB; ++v) {
+                    const int c = column<VW, TPR, VPT>(t, v0 + v);
                     uint32_t b[VW];
 #pragma unroll
                     for (int i = 0; i < VW; ++i)
-                        b[i] = eight_round((double)h[v][i], (double)up);
+                        b[i] = eight_round(y[v][i], (double)up);
                     if (c < a.pitch) {  // columns between dim and the pitch hold zeros
                         if constexpr (VW == 8)
                             *reinterpret_cast<uint2 *>(q + c) =
@@ -222,41 +221,50 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs
 template <typename T, bool EIGHT>
 __global__ void __launch_bounds__(1024) norm_wide_kernel(const NormArgs a)
 {
-    using H = typename std::conditional<EIGHT, double, float>::type;
     __shared__ double sums[32];
     const T *w = static_cast<const T *>(a.w);
     for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
         const T *x = static_cast<const T *>(a.x) + row * a.ld_x;
         const T *r = a.r ? static_cast<const T *>(a.r) + row * a.ld_r : nullptr;
-        double ss = 0;
+        double ss = 0, ss64 = 0;
         for (int c = threadIdx.x; c < a.dim; c += 1024) {
-            const H h = r ? (H)to_float(x[c]) + (H)to_float(r[c]) : (H)to_float(x[c]);
+            const float xi = to_float(x[c]), ri = r ? to_float(r[c]) : 0.f;
+            const float h = r ? xi + ri : xi;
+            const double h64 = r ? (double)xi + (double)ri : (double)xi;
             ss = fma((double)h, (double)h, ss);
+            ss64 = fma(h64, h64, ss64);
         }
         ss = row_sum<double, 1024>(ss, PSPMM_FULL_MASK, sums);
-        const double rstd64 = 1.0 / sqrt(ss / a.dim + a.eps);
-        const H rstd = (H)rstd64;
+        const float rstd = (float)(1.0 / sqrt(ss / a.dim + a.eps));
         if (threadIdx.x == 0)
-            a.rstd[row] = (float)rstd64;
+            a.rstd[row] = rstd;
+        double rstd64 = 0;
+        if constexpr (EIGHT)
+            rstd64 = 1.0 / sqrt(row_sum<double, 1024>(ss64, PSPMM_FULL_MASK, sums) / a.dim + a.eps);
         // A warp takes 128 neighbouring columns at a time, a lane four of them.
         for (int c0 = threadIdx.x * 4; c0 < (a.dim + EIGHT_BLOCK - 1) / EIGHT_BLOCK * EIGHT_BLOCK; c0 += 4096) {
-            H y[4];
+            double y64[4];
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int c = c0 + i;
-                y[i] = (H)0;
+                y64[i] = 0;
                 if (c < a.dim) {
-                    const H h = r ? (H)to_float(x[c]) + (H)to_float(r[c]) : (H)to_float(x[c]);
-                    y[i] = h * rstd * (H)to_float(w[c]);
-                    if (a.relu && y[i] < (H)0)
-                        y[i] = (H)0;
+                    const float xi = to_float(x[c]), ri = r ? to_float(r[c]) : 0.f, wi = to_float(w[c]);
+                    const float h = r ? xi + ri : xi;
                     if (a.h)
-                        static_cast<T *>(a.h)[row * a.ld_h + c] = from_float<T>((float)h);
-                    if (a.y)
-                        static_cast<T *>(a.y)[row * a.ld_y + c] = from_float<T>((float)y[i]);
+                        static_cast<T *>(a.h)[row * a.ld_h + c] = from_float<T>(h);
+                    if (a.y) {
+                        const float y = h * rstd * wi;
+                        static_cast<T *>(a.y)[row * a.ld_y + c] = from_float<T>(a.relu && y < 0.f ? 0.f : y);
+                    }
+                    if constexpr (EIGHT) {
+                        y64[i] = (r ? (double)xi + (double)ri : (double)xi) * rstd64 * (double)wi;
+                        if (a.relu && y64[i] < 0.0)
+                            y64[i] = 0.0;
+                    }
                 }
-                top = max(top, __float_as_uint((float)y[i]) & 0x7fffffffu);
+                top = max(top, __float_as_uint((float)y64[i]) & 0x7fffffffu);
             }
             if constexpr (EIGHT) {
                 top = __reduce_max_sync(PSPMM_FULL_MASK, top);
@@ -267,7 +275,7 @@ __global__ void __launch_bounds__(1024) norm_wide_kernel(const NormArgs a)
                 uint32_t b[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    b[i] = eight_round((double)y[i], (double)up);
+                    b[i] = eight_round(y64[i], (double)up);
                 if (c0 < a.pitch)
                     *reinterpret_cast<uint32_t *>(a.q + row * a.pitch + c0) = pack_bytes(b[0], b[1], b[2], b[3]);
             }

@@ -167,6 +167,10 @@ class Rows8:
             check(rc)
         return out
 
+    def weight_grad(self, G):
+        """:func:`rows8_mm_t` of these rows and ``G``."""
+        return rows8_mm_t(self, G)
+
 
 def _empty_rows8(n, dim, device):
     return (torch.empty((n, dim + -dim % 16), dtype=torch.int8, device=device),

@@ -10,14 +10,19 @@ Same module and autograd-function names, constructor arguments and forward signa
 * AGNN  forward  X' = X W, e = SDDMM(X', X') * beta, out = SpMM(e, X'); no edge softmax and no
         row normalisation (the reference has none); the gradient w.r.t. beta follows the
         reference's expression (gnn_conv.py:164-172).
+
+Beside them stand two layers that the reference does not have, ``NodeEmbedding`` (learned features of graphs that come without)
+and ``RMSNorm`` (the residual stream of deep networks), and a layer can keep its input for the backward in 8 bits
+(``keep_input_8bit``, or the 8-bit form that an ``RMSNorm`` left, as ``kept``).
 """
 from __future__ import annotations
 
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
-from . import ops
+from . import feature_ops, ops
 
 n_heads = 1
 
@@ -38,16 +43,32 @@ def _aggregate(P, X):
     return out[: X.shape[0]] if out.shape[0] != X.shape[0] else out  # block layouts pad the row count
 
 
+def _save(ctx, kept, *others):
+    """What the backward needs: the factor of the weight gradient, as a tensor or in 8 bits, and ``others``."""
+    ctx.kept_dim = None if isinstance(kept, torch.Tensor) else kept.dim
+    ctx.save_for_backward(*((kept,) if ctx.kept_dim is None else (kept.q, kept.scales)), *others)
+
+
+def _saved(ctx):
+    t = ctx.saved_tensors
+    return t if ctx.kept_dim is None else (feature_ops.Rows8(t[0], t[1], ctx.kept_dim), *t[2:])
+
+
+def _held(X, eight):
+    """``X`` as the backward is to have it: itself, or in 8 bits (``eight``: True, or those bits)."""
+    return X if eight is None else feature_ops.quantize_rows(X) if eight is True else eight
+
+
 class GCNFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, H, weight, ParamSpMM):
+    def forward(ctx, H, weight, ParamSpMM, eight=None):
         ctx.ParamSpMM = ParamSpMM
         ctx.narrow_first = bool(REORDER_NARROW_FIRST and weight.shape[0] < weight.shape[1])
         if ctx.narrow_first:
             AH = _aggregate(ParamSpMM, H)
-            ctx.save_for_backward(AH, weight)
+            _save(ctx, _held(AH, None if eight is None else True), weight)
             return torch.mm(AH, weight)
-        ctx.save_for_backward(H, weight)
+        _save(ctx, _held(H, eight), weight)
         return ParamSpMM.forward(H, weight)
 
     @staticmethod
@@ -57,32 +78,32 @@ class GCNFunction(torch.autograd.Function):
         if ctx.narrow_first:
             # dW = (A H)^T G with A H kept from the forward; dH = A (G W^T) (A is symmetric),
             # skipped when the layer input needs no gradient (the first layer).
-            AH, weight = ctx.saved_tensors
-            d_weight = ops.dense_mm(AH, d_output, transA=True)
+            AH, weight = _saved(ctx)
+            d_weight = ops._weight_grad(AH, d_output)
             d_input = _aggregate(P, ops.dense_mm(d_output, weight, transB=True)) if ctx.needs_input_grad[0] else None
-            return d_input, d_weight, None
-        H, weight = ctx.saved_tensors
+            return d_input, d_weight, None, None
+        H, weight = _saved(ctx)
         if ctx.needs_input_grad[0]:
             d_input, d_weight = P.backward(d_output, H, weight)
         else:  # the first layer: dH = AG W^T is not formed (the reference forms and drops it)
             d_input, d_weight = P.backward(d_output, H, weight, input_grad=False)
-        return d_input, d_weight, None
+        return d_input, d_weight, None, None
 
 
 class GINFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, X, weight, ParamSpMM):
+    def forward(ctx, X, weight, ParamSpMM, eight=None):
         X_agg = ParamSpMM.GIN_spmm(X)
-        ctx.save_for_backward(X_agg, weight)
+        _save(ctx, _held(X_agg, eight), weight)
         ctx.ParamSpMM = ParamSpMM
         return torch.mm(X_agg, weight)
 
     @staticmethod
     def backward(ctx, d_output):
-        X_agg, weight = ctx.saved_tensors
-        d_weight = ops.dense_mm(X_agg, d_output, transA=True)
+        X_agg, weight = _saved(ctx)
+        d_weight = ops._weight_grad(X_agg, d_output)
         d_input = ctx.ParamSpMM.GIN_spmm(ops.dense_mm(d_output, weight, transB=True).contiguous())
-        return d_input, d_weight, None
+        return d_input, d_weight, None, None
 
 
 # Under torch.no_grad() an AGNN layer on a plain or split CSR operator runs as the fused kernel
@@ -148,29 +169,29 @@ def _same_entries(colIdx, own):
 
 class AGNNFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, X, weights, attention_w, ParamSpMM, colIdx):
+    def forward(ctx, X, weights, attention_w, ParamSpMM, colIdx, eight=None):
         X_prime = ops.dense_mm(X, weights)
         edge = ParamSpMM.AGNN_sddmm(X_prime)
         # [n_edges] for CSR, [n_blocks, V] for block layouts; one attention head
         edge_attentions = (edge * attention_w.reshape(())).contiguous()
         out = ParamSpMM.AGNN_spmm(edge_attentions, X_prime)
-        ctx.save_for_backward(X, weights, edge_attentions)
+        _save(ctx, _held(X, eight), weights, edge_attentions)
         ctx.colIdx, ctx.ParamSpMM = colIdx, ParamSpMM
         return out
 
     @staticmethod
     def backward(ctx, d_output):
         P = ctx.ParamSpMM
-        X, weights, edge_attentions = ctx.saved_tensors
+        X, weights, edge_attentions = _saved(ctx)
         d_output = d_output.contiguous()
         d_prime = P.AGNN_spmm(edge_attentions, d_output)
         d_input = ops.dense_mm(d_prime, weights, transB=True)
-        d_weights = ops.dense_mm(X, d_prime, transA=True)
+        d_weights = ops._weight_grad(X, d_prime)
         d_att = P.AGNN_sddmm(d_output)
         if d_att.dim() != 1:
             d_att = d_att.reshape(-1)[P.mask]  # back to CSR entry order
         d_attention_w = torch.mm(d_att[None, :].expand(n_heads, -1), ctx.colIdx.float()).transpose(0, 1)
-        return d_input, d_weights, d_attention_w, None, None
+        return d_input, d_weights, d_attention_w, None, None, None
 
 
 class AGNNFusedFunction(torch.autograd.Function):
@@ -187,7 +208,7 @@ class AGNNFusedFunction(torch.autograd.Function):
     Like the reference's backward, the edge values are treated as constants with respect to X'."""
 
     @staticmethod
-    def forward(ctx, X, weights, attention_w, P, colIdx, keep_scores=True):
+    def forward(ctx, X, weights, attention_w, P, colIdx, keep_scores=True, eight=None):
         Xp = ops.dense_mm(X, weights)
         beta, scores = _beta(attention_w), None
         if keep_scores and _keeps_scores(P.colIdx.shape[0], Xp):
@@ -198,23 +219,111 @@ class AGNNFusedFunction(torch.autograd.Function):
         if scores is None:
             beta = beta.clone()  # (the backward uses the value of this forward)
         out = ops.agnn_layer_forward(Xp, P.rowPtr, P.colIdx, beta, P.target_row, scores)
-        ctx.save_for_backward(X, weights, *((Xp, beta) if scores is None else (scores,)))
+        _save(ctx, _held(X, eight), weights, *((Xp, beta) if scores is None else (scores,)))
         ctx.P = P
         return out
 
     @staticmethod
     def backward(ctx, d_output):
-        X, weights, *rest = ctx.saved_tensors
+        X, weights, *rest = _saved(ctx)
         Xp, beta, scores = (*rest, None) if len(rest) == 2 else (None, None, *rest)
         P = ctx.P
         D, d_att = ops.agnn_layer_backward(Xp, d_output.contiguous(), P.rowPtr, P.colIdx, beta, P.target_row,
                                            beta_grad=ctx.needs_input_grad[2], scores=scores)
         d_input = ops.dense_mm(D, weights, transB=True) if ctx.needs_input_grad[0] else None
-        d_weights = ops.dense_mm(X, D, transA=True) if ctx.needs_input_grad[1] else None
-        return d_input, d_weights, d_att, None, None, None
+        d_weights = ops._weight_grad(X, D) if ctx.needs_input_grad[1] else None
+        return d_input, d_weights, d_att, None, None, None, None
+
+
+class EmbeddingFunction(torch.autograd.Function):
+    """scale * table[ids]; the table's gradient is dense, sums over equal ids in the order of their positions."""
+
+    @staticmethod
+    def forward(ctx, ids, table, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.args = (table.shape[0], scale, padding_idx)
+        return feature_ops.embedding(ids, table, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        ids, = ctx.saved_tensors
+        return None, feature_ops.embedding_grad(ids, grad.contiguous(), *ctx.args), None, None
+
+
+class RMSNormFunction(torch.autograd.Function):
+    """(y, h, q, scales) of ``feature_ops.rms_norm``; h is None without a residual, q and scales without ``eight_bit``.  Kept for the
+    backward: h and one float per row."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, relu, eight_bit):
+        y, h, rstd, kept = feature_ops.rms_norm(x, weight, residual, eps, relu, eight_bit=eight_bit)
+        ctx.save_for_backward(h, rstd, weight)
+        ctx.relu, ctx.stream = relu, residual is not None
+        ctx.set_materialize_grads(False)
+        q, scales = (kept.q, kept.scales) if eight_bit else (None, None)
+        if eight_bit:
+            ctx.mark_non_differentiable(q, scales)
+        return y, h if ctx.stream else None, q, scales
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh, _q, _scales):
+        h, rstd, weight = ctx.saved_tensors
+        if dy is None:  # only the residual stream went on
+            return dh, dh if ctx.stream else None, None, None, None, None
+        dx, dw = feature_ops.rms_norm_backward(dy.contiguous(), h, rstd, weight, None if dh is None else dh.contiguous(), ctx.relu)
+        return dx, dx if ctx.stream else None, dw, None, None, None
+
+
+class NodeEmbedding(torch.nn.Module):
+    """Learned features: ``scale * weights[ids]`` for graphs whose nodes have none.  ``padding_idx`` names a row that takes no
+    gradient (ids that fill up a batch)."""
+
+    def __init__(self, n_rows, dim, scale=1.0, padding_idx=None):
+        super().__init__()
+        if padding_idx is not None and not 0 <= padding_idx < n_rows:
+            raise ValueError("padding_idx must be a row of the table")
+        self.scale, self.padding_idx = scale, padding_idx
+        self.weights = torch.nn.Parameter(torch.empty(n_rows, dim))
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        stdv = 1.0 / math.sqrt(self.weights.size(1))
+        self.weights.data.uniform_(-stdv, stdv)
+        if self.padding_idx is not None:
+            self.weights.data[self.padding_idx] = 0
+
+    def forward(self, ids):
+        return EmbeddingFunction.apply(ids, self.weights, self.scale, self.padding_idx)
+
+
+class RMSNorm(torch.nn.Module):
+    """Root-mean-square norm of ``x + residual``, then relu where asked for: the step between the layers of a deep network,
+
+        y, h = norm(conv_out, h)              # h: the residual stream
+        y, h, kept = norm(conv_out, h, eight_bit=True)
+        conv_out = conv(y, spmm_dict, kept)   # the layer keeps those 8 bits for its backward instead of y
+
+    The backward keeps h, so that with relu in here and the next layer's input in 8 bits nothing else of this step lives on."""
+
+    def __init__(self, dim, eps=1e-6, relu=False):
+        super().__init__()
+        self.eps, self.relu = eps, relu
+        self.weights = torch.nn.Parameter(torch.ones(dim))
+
+    def forward(self, x, residual=None, eight_bit=False):
+        y, h, q, scales = RMSNormFunction.apply(x, residual, self.weights, self.eps, self.relu, eight_bit)
+        h = x if residual is None else h
+        return (y, h, feature_ops.Rows8(q, scales, x.shape[-1], x.shape)) if eight_bit else (y, h)
 
 
 class _Conv(torch.nn.Module):
+    # True: what a layer keeps for its weight gradient (its input; GIN: the aggregated one) is kept in 8 bits, a scale per row and 128
+    # columns, and the gradient is formed from those: a quarter of the memory, off by at most 1/254 of the largest value that
+    # shares the scale
+    keep_input_8bit = False
+
     def __init__(self, input_dim, output_dim):
         super().__init__()
         self.weights = torch.nn.Parameter(torch.randn(input_dim, output_dim))
@@ -230,18 +339,26 @@ class _Conv(torch.nn.Module):
             raise ValueError("SpMMDecider not support dim: " + str(dim))
         return spmm_dict[dim]
 
+    def _eight(self, X, kept):
+        """``kept`` where the caller has the input in 8 bits, True where it is to be made, None where it is kept as it is."""
+        if kept is None:
+            return True if self.keep_input_8bit and torch.is_grad_enabled() else None
+        if not isinstance(kept, feature_ops.Rows8) or kept.shape != X.shape or kept.q.device != X.device:
+            raise RuntimeError("kept must be the layer's input in 8 bits")
+        return kept
+
 
 class GCNConv(_Conv):
-    def forward(self, H, spmm_dict):
+    def forward(self, H, spmm_dict, kept=None):
         P = self._operator(spmm_dict)
         if REORDER_NARROW_FIRST and self.weights.size(0) < self.weights.size(1):
             P = spmm_dict.get(self.weights.size(0), P)  # the aggregation runs at the input width
-        return GCNFunction.apply(H, self.weights, P)
+        return GCNFunction.apply(H, self.weights, P, self._eight(H, kept))
 
 
 class GINConv(_Conv):
     def forward(self, X, spmm_dict):
-        return GINFunction.apply(X, self.weights, self._operator(spmm_dict))
+        return GINFunction.apply(X, self.weights, self._operator(spmm_dict), self._eight(X, None))
 
 
 class AGNNConv(_Conv):
@@ -253,7 +370,7 @@ class AGNNConv(_Conv):
         super().__init__(input_dim, output_dim)
         self.attention_w = torch.nn.Parameter(torch.randn(1, n_heads))
 
-    def forward(self, X, spmm_dict, colIdx):
+    def forward(self, X, spmm_dict, colIdx, kept=None):
         P = self._operator(spmm_dict)
         if FUSE_AGNN_INFERENCE and not torch.is_grad_enabled() and _can_fuse(P, self.weights.size(1)):
             # No gradient will be asked for: scores, scaling and aggregation in one kernel, without
@@ -261,7 +378,8 @@ class AGNNConv(_Conv):
             Xp = ops.dense_mm(X, self.weights)
             out = ops.agnn_layer_forward(Xp, P.rowPtr, P.colIdx, _beta(self.attention_w), P.target_row)
             return out[: P.mtx_nodes if P.target_row is not None else P.rowPtr.shape[0] - 1]
+        eight = self._eight(X, kept)
         if (FUSE_AGNN_TRAINING and torch.is_grad_enabled() and _can_fuse(P, self.weights.size(1))
                 and _is_operator_colidx(P, colIdx)):
-            return AGNNFusedFunction.apply(X, self.weights, self.attention_w, P, colIdx, self.keep_scores)
-        return AGNNFunction.apply(X, self.weights, self.attention_w, P, colIdx)
+            return AGNNFusedFunction.apply(X, self.weights, self.attention_w, P, colIdx, self.keep_scores, eight)
+        return AGNNFunction.apply(X, self.weights, self.attention_w, P, colIdx, eight)

@@ -888,6 +888,11 @@ def dense_mm(A, B, transA=False, transB=False, out=None):
     return out
 
 
+def _weight_grad(H, G):
+    """H^T G, H as a layer kept it: a tensor, or rows in 8 bits (``feature_ops.Rows8``)."""
+    return dense_mm(H, G, transA=True) if isinstance(H, torch.Tensor) else H.weight_grad(G)
+
+
 def dense_status():
     """1 once a bounded wait of the dense product has run out in this process, else 0 (synchronises with the
     device).  The rows of the result that were not computed are NaN then."""
@@ -921,7 +926,7 @@ def _conv_forward(V, H, weight, rowPtr, colIdx, val, target_row, CF, W, product=
 
 def _conv_backward(V, g_out, H, weight, rowPtr, colIdx, val, target_row, CF, W, product=None, input_grad=True):
     """AG = A @ g_out (A itself, the normalised adjacency is symmetric); dH = AG @ W^T;
-    dW = H^T @ AG (SpCONV/SpCONV.h:57-72).  Odd widths are padded as in the forward.
+    dW = H^T @ AG (SpCONV/SpCONV.h:57-72).  Odd widths are padded as in the forward.  ``H`` may be held in 8 bits.
     ``input_grad=False`` leaves dH out (None): the first layer of a network has no use for it."""
     _check_legacy(CF, W, max_cf=4)
     n, fout = g_out.shape
@@ -931,7 +936,7 @@ def _conv_backward(V, g_out, H, weight, rowPtr, colIdx, val, target_row, CF, W, 
         g_out = _pad_cols(g_out, -fout % 4).contiguous()
     AG = product(g_out) if product else _spmm(g_out, rowPtr, colIdx, val, target_row, V, CF, W)
     AG = AG[:n, :fout]
-    d_weight = dense_mm(H, AG, transA=True)
+    d_weight = _weight_grad(H, AG)
     d_input = dense_mm(AG, weight, transB=True) if input_grad else None
     return [d_input, d_weight]
 
