@@ -407,12 +407,15 @@ PSPMM_API int pspmm_dequantize_rows(const int8_t *q, int64_t pitch, const float 
 /*
  * C[dim, cols] = X^T G, fp32, where X[n, dim] is held in the 8-bit form (q, scales) and G[n, cols] has element type dtype: the weight
  * gradient of a layer that kept its input in 8 bits.  On the tensor cores with fp32 accuracy: q is exact in bf16, scale * G (rounded
- * to fp32) is cut into three bf16 parts whose sum it is.  Any size and alignment of G.  Scratch:
- * pspmm_rows8_mm_t_scratch_bytes(n, dim, cols) bytes, 16-byte aligned.  n == 0 gives zeros.  Waits inside the kernel are bounded (two
+ * to fp32) is cut into three bf16 parts whose sum it is.  Any size and alignment of G.  Scratch, 16-byte aligned:
+ * pspmm_rows8_mm_t_scratch_bytes(n, dim, cols, dtype, 1) bytes are required; aligned = 0, for a G whose rows do not all start on 16
+ * bytes, adds room for a copy of G whose rows do, without which such a product takes two to three times as long.  n == 0 gives
+ * zeros.  Waits inside the kernel are bounded (two
  * seconds): when one runs out, what was not computed of C becomes NaN and pspmm_rows8_mm_status returns 1 from then on in this
  * process (it synchronises).  pspmm_rows8_mm_t_stalled is for tests of that path, as pspmm_dense_mm_stalled.
  */
-PSPMM_API int pspmm_rows8_mm_t_scratch_bytes(int64_t n, int32_t dim, int32_t cols, size_t *bytes);
+PSPMM_API int pspmm_rows8_mm_t_scratch_bytes(int64_t n, int32_t dim, int32_t cols, int32_t dtype, int32_t aligned,
+                                             size_t *bytes);
 PSPMM_API int pspmm_rows8_mm_t(const int8_t *q, int64_t pitch, const float *scales, int64_t n, int32_t dim, const void *G,
                                int32_t dtype, int64_t ldG, int32_t cols, float *C, int64_t ldC, void *scratch,
                                size_t scratch_bytes, void *stream);

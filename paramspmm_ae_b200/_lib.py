@@ -119,7 +119,7 @@ _SIGNATURES = {
     "pspmm_dense_status": [ctypes.POINTER(ctypes.c_int32)],
     "pspmm_quantize_rows": [_vp, _i32, _i64, _i64, _i32, _vp, _i64, _vp, _vp],
     "pspmm_dequantize_rows": [_vp, _i64, _vp, _i32, _vp, _i64, _i64, _i32, _vp],
-    "pspmm_rows8_mm_t_scratch_bytes": [_i64, _i32, _i32, ctypes.POINTER(ctypes.c_size_t)],
+    "pspmm_rows8_mm_t_scratch_bytes": [_i64, _i32, _i32, _i32, _i32, ctypes.POINTER(ctypes.c_size_t)],
     "pspmm_rows8_mm_t": [_vp, _i64, _vp, _i64, _i32, _vp, _i32, _i64, _i32, _vp, _i64, _vp, ctypes.c_size_t, _vp],
     "pspmm_rows8_mm_t_stalled": [_vp, _i64, _vp, _i64, _i32, _vp, _i32, _i64, _i32, _vp, _i64, _vp, ctypes.c_size_t, _vp],
     "pspmm_rows8_mm_status": [ctypes.POINTER(ctypes.c_int32)],

@@ -19,7 +19,8 @@
 // stages under way to shared memory of its own, as it lies: tiles by TMA, or words by cp.async where G's rows are not aligned.  (Loads
 // to registers that are to outlast a stage are waited for together with the next ones, however they are ordered.)  Two warps
 // issue the MMAs; eight add finished chains out of TMEM (two buffers of 128 columns) and store the tile.  Ranges of rows leave
-// partial tiles in scratch, which reduce_kernel adds in order.
+// partial tiles in scratch, which reduce_kernel adds in order.  G with unaligned rows is copied to aligned ones first where scratch
+// has room for it.
 //
 // An infinity of x keeps its sign (its lower parts are zeros), a NaN stays one.  Parts below 2^-133, bf16's least, are lost.
 //
@@ -50,8 +51,8 @@ constexpr int GROUP_WARPS = 4, LOADERS = GROUPS * GROUP_WARPS, DRAINERS = 8;
 constexpr int MMA_WARP = LOADERS + DRAINERS;
 constexpr int THREADS = (LOADERS + DRAINERS + 4) * 32;
 constexpr int TMEM_X = ACC_BUFS * BM, TMEM_COLS = 512;  // the parts of x: 16 columns each, 48 per slot
-// Registers per thread after the split: 896 x 72 = 64,512 at launch; 512 x 72 + 256 x 88 + 128 x 32 = 63,488.
-constexpr int DRAINER_REGS = 88, OTHER_REGS = 32;
+// Registers per thread after the split: 896 x 72 = 64,512 at launch; 512 x 72 + 256 x 88 + 128 x 40 = 64,512.
+constexpr int DRAINER_REGS = 88, OTHER_REGS = 40;
 // What a warp brings in per stage, as it lies in memory: 32 columns of 32 rows of G (by words: one more than fills them, for rows that
 // begin inside a word), 8 rows of q, 32 scales.
 template <typename T, bool TMA> struct Raw {
@@ -124,13 +125,11 @@ __device__ __forceinline__ void acc_load8(uint32_t (&v)[8], uint32_t addr)
                  : "r"(addr));
 }
 
-// One part (16 packed columns) of the warp's 32 columns of G -> TMEM.
-__device__ __forceinline__ void part_store(uint32_t addr, const uint32_t (&v)[16])
+// Half a part (8 packed columns) of the warp's 32 columns of G -> TMEM.
+__device__ __forceinline__ void part_store(uint32_t addr, const uint32_t (&v)[8])
 {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-                 "%14, %15, %16};"
-                 ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-                 "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
 
@@ -191,32 +190,28 @@ __device__ __forceinline__ void copy_tile(uint32_t dst, const CUtensorMap *map, 
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 template <int PENDING> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
-// A thread's 32 rows of its column -> three parts in TMEM.  False if a value has no split: the remainder of an infinity or a NaN is
-// a NaN.
-__device__ __forceinline__ bool split_column(pair_t (&x)[BK / 2], uint32_t addr)
+// 16 rows of a thread's column -> half of each part in TMEM.  What is left of an infinity or a NaN is a NaN: `rest` adds up the
+// remainders, so that one look at it tells whether all values had a split.
+__device__ __forceinline__ void split_column(pair_t (&x)[8], uint32_t addr, pair_t &rest)
 {
-    uint32_t v[BK / 2];
-    pair_t rest = 0;
+    uint32_t v[8];
 #pragma unroll
-    for (int i = 0; i < BK / 2; ++i) {
+    for (int i = 0; i < 8; ++i) {
         v[i] = cut_pair(x[i]);
         rest = add_pair(rest, x[i]);
     }
     part_store(addr, v);
 #pragma unroll
-    for (int i = 0; i < BK / 2; ++i)
+    for (int i = 0; i < 8; ++i)
         v[i] = cut_pair(x[i]);
     part_store(addr + 16, v);
 #pragma unroll
-    for (int i = 0; i < BK / 2; ++i) {
+    for (int i = 0; i < 8; ++i) {
         float x0, x1;
         get_pair(x[i], x0, x1);
         v[i] = __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
     }
     part_store(addr + 32, v);
-    float r0, r1;
-    get_pair(rest, r0, r1);
-    return r0 + r1 == r0 + r1;
 }
 // The parts of a value of any kind: an infinity stands in the upper part alone, and a NaN is one there.
 __device__ __forceinline__ uint32_t part_of(float x, int part)
@@ -290,6 +285,8 @@ __global__ void __launch_bounds__(THREADS, 1) rows8_mm_kernel(const MmArgs a, co
         // Words: even and odd rows of a stage begin this far into one, the same in every stage.
         const int off[2] = {TMA || SZ == 4 ? 0 : (int)((g_col + i0 * g_row) & 2), TMA || SZ == 4 ? 0 : (int)((g_col + (i0 + 1) * g_row) & 2)};
 
+        const float *sp = a.scales + (i0 + g * BK + lane) * a.blocks + mt;  // of the next stage's rows
+
         auto fetch = [&](int s, int buf) {
             if (s < stages) {
                 const uint32_t raw = raw0 + buf * R::BYTES;
@@ -328,7 +325,8 @@ __global__ void __launch_bounds__(THREADS, 1) rows8_mm_kernel(const MmArgs a, co
                     }
                 }
                 const bool in = i + lane < i1;
-                copy4(raw + R::SCALES + lane * 4, a.scales + (in ? (i + lane) * a.blocks + mt : 0), in ? 4 : 0);
+                copy4(raw + R::SCALES + lane * 4, in ? sp : a.scales, in ? 4 : 0);
+                sp += (int64_t)a.blocks * (GROUPS * BK);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");  // (an empty one keeps the count)
         };
@@ -367,14 +365,22 @@ __global__ void __launch_bounds__(THREADS, 1) rows8_mm_kernel(const MmArgs a, co
                     make_uint4(bf16_pair(v.x, 0x4140), bf16_pair(v.x, 0x4342), bf16_pair(v.y, 0x4140), bf16_pair(v.y, 0x4342));
             }
             if (some) {
-                pair_t x[BK / 2];
+                pair_t rest = 0;
 #pragma unroll
-                for (int k = 0; k < BK; k += 4) {
-                    const float4 v = *reinterpret_cast<const float4 *>(raw + R::SCALES + k * 4);
-                    x[k / 2] = mul_pair(make_pair(value(raw, k), value(raw, k + 1)), make_pair(v.x, v.y));
-                    x[k / 2 + 1] = mul_pair(make_pair(value(raw, k + 2), value(raw, k + 3)), make_pair(v.z, v.w));
+                for (int half = 0; half < 2; ++half) {
+                    pair_t x[8];
+#pragma unroll
+                    for (int k = 0; k < 16; k += 4) {
+                        const int row = half * 16 + k;
+                        const float4 v = *reinterpret_cast<const float4 *>(raw + R::SCALES + row * 4);
+                        x[k / 2] = mul_pair(make_pair(value(raw, row), value(raw, row + 1)), make_pair(v.x, v.y));
+                        x[k / 2 + 1] = mul_pair(make_pair(value(raw, row + 2), value(raw, row + 3)), make_pair(v.z, v.w));
+                    }
+                    split_column(x, lanes_x + slot * 48 + half * 8, rest);
                 }
-                if (!__all_sync(PSPMM_FULL_MASK, split_column(x, lanes_x + slot * 48)))
+                float rest0, rest1;
+                get_pair(rest, rest0, rest1);
+                if (__any_sync(PSPMM_FULL_MASK, rest0 + rest1 != rest0 + rest1))
                     store_slowly(raw, lanes_x + slot * 48);
             }
             __syncwarp();
@@ -510,6 +516,36 @@ __global__ void __launch_bounds__(THREADS, 1) rows8_mm_kernel(const MmArgs a, co
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
 }
 
+struct PadArgs {
+    const void *src;
+    void *dst;
+    int64_t rows, ld, pitch;
+    int32_t cols;
+};
+
+// Rows of G moved to 16-byte boundaries, zeros behind them: a warp takes four rows at a time.
+template <typename T> __global__ void __launch_bounds__(256) pad_kernel(const PadArgs a)
+{
+    const int lane = threadIdx.x & 31;
+    const int64_t warps = (int64_t)gridDim.x * 8;
+    for (int64_t r0 = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r0 < a.rows; r0 += 4 * warps) {
+        for (int c = lane; c < a.pitch; c += 32) {
+            T v[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int64_t r = r0 + t * warps;
+                v[t] = r < a.rows && c < a.cols ? static_cast<const T *>(a.src)[r * a.ld + c] : from_float<T>(0.f);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int64_t r = r0 + t * warps;
+                if (r < a.rows)
+                    static_cast<T *>(a.dst)[r * a.pitch + c] = v[t];
+            }
+        }
+    }
+}
+
 // C = sum of the partial tiles: a block takes 32 neighbouring elements, its eight warps the splits in turn.
 __global__ void __launch_bounds__(256) reduce_kernel(const ReduceArgs a)
 {
@@ -568,8 +604,11 @@ void plan(int64_t rows, int32_t M, int32_t N, MmArgs &a)
 
 size_t partial_bytes(const MmArgs &a, int32_t M, int32_t N)
 {
-    return a.splits > 1 ? (size_t)a.splits * (size_t)M * (size_t)N * sizeof(float) : 0;
+    return a.splits > 1 ? ((size_t)a.splits * (size_t)M * (size_t)N * sizeof(float) + 255) / 256 * 256 : 0;
 }
+// A copy of G with rows of whole 16 bytes.
+int64_t padded_cols(int32_t N, int bytes) { return ((int64_t)N * bytes + 15) / 16 * 16 / bytes; }
+size_t padded_bytes(int64_t rows, int32_t N, int bytes) { return (size_t)rows * (size_t)padded_cols(N, bytes) * bytes; }
 
 // The driver's function that describes an array to TMA (the library links the runtime only); null where there is none.
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -613,8 +652,18 @@ template <typename T, bool TMA> cudaError_t launch_loads(const MmArgs &a, const 
 }
 
 // Tiles by TMA where the rows of both operands begin on 16 bytes (its strides are below 2^40 and its coordinates 32 bits).
-template <typename T> cudaError_t launch(const MmArgs &a, cudaStream_t st)
+template <typename T> cudaError_t launch(MmArgs a, void *padded, cudaStream_t st)
 {
+    if (padded) {
+        const PadArgs p = {a.G, padded, a.rows, a.ldG, padded_cols(a.N, sizeof(T)), a.N};
+        const int64_t ctas = (a.rows + 31) / 32, most = (int64_t)pspmm_sm_count() * 16;
+        pad_kernel<T><<<(unsigned)(ctas < most ? ctas : most), 256, 0, st>>>(p);
+        cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess)
+            return e;
+        a.G = padded;
+        a.ldG = p.pitch;
+    }
     Maps maps = {};
     if (rows_aligned(a.G, a.ldG, sizeof(T), 16) && a.rows < INT32_MAX - 1024 && a.ldG * (int64_t)sizeof(T) < 1ll << 40 && encode_tiled() &&
         describe(maps.G, a.G, sizeof(T), a.N, a.rows, a.ldG, 32, BK) && describe(maps.q, a.q, 1, a.pitch, a.rows, a.pitch, BM, 8))
@@ -662,9 +711,13 @@ int mm_run(const int8_t *q, int64_t pitch, const float *scales, int64_t rows, in
     a.blocks = (dim + EIGHT_BLOCK - 1) / EIGHT_BLOCK;
     a.wait_ns = wait_ns;
     a.withhold = withhold;
-    PSPMM_CUDA_TRY(dtype == PSPMM_F32    ? launch<float>(a, st)
-                   : dtype == PSPMM_BF16 ? launch<bf16>(a, st)
-                                         : launch<f16>(a, st));
+    const int B = elem_bytes(dtype);
+    void *padded = nullptr;  // (scratch that has no room for the copy is used without it)
+    if (!rows_aligned(G, ldG, B, 16) && scratch && scratch_bytes >= need + padded_bytes(rows, cols, B) && (uintptr_t)scratch % 16 == 0)
+        padded = (char *)scratch + need;
+    PSPMM_CUDA_TRY(dtype == PSPMM_F32    ? launch<float>(a, padded, st)
+                   : dtype == PSPMM_BF16 ? launch<bf16>(a, padded, st)
+                                         : launch<f16>(a, padded, st));
     if (a.splits > 1) {
         const ReduceArgs r = {a.C, C, ldC, a.splits, dim, cols};
         PSPMM_CUDA_TRY(launch_dependent(reduce_kernel, dim3((unsigned)(((int64_t)dim * cols + 31) / 32)), 256, 0, st, r));
@@ -674,16 +727,16 @@ int mm_run(const int8_t *q, int64_t pitch, const float *scales, int64_t rows, in
 
 }  // namespace
 
-extern "C" int pspmm_rows8_mm_t_scratch_bytes(int64_t n, int32_t dim, int32_t cols, size_t *bytes)
+extern "C" int pspmm_rows8_mm_t_scratch_bytes(int64_t n, int32_t dim, int32_t cols, int32_t dtype, int32_t aligned, size_t *bytes)
 {
-    if (n < 0 || dim < 1 || cols < 0 || !bytes)
+    if (n < 0 || dim < 1 || cols < 0 || !dtype_ok(dtype) || !bytes)
         return PSPMM_E_ARG;
     *bytes = 0;
     if (n == 0 || cols == 0)
         return PSPMM_OK;
     MmArgs a = {};
     plan(n, dim, cols, a);
-    *bytes = partial_bytes(a, dim, cols);
+    *bytes = partial_bytes(a, dim, cols) + (aligned ? 0 : padded_bytes(n, cols, elem_bytes(dtype)));
     return PSPMM_OK;
 }
 

@@ -207,7 +207,14 @@ def rows8_mm_t(rows, G, out=None):
         out = torch.empty((rows.dim, cols), dtype=torch.float32, device=G.device)
     elif (out.dtype is not torch.float32 or out.shape != (rows.dim, cols) or out.stride(1) != 1 or out.stride(0) < cols):
         raise RuntimeError("out must be a float32 matrix of %d rows of %d with unit column stride" % (rows.dim, cols))
-    scratch, need = _scratch("pspmm_rows8_mm_t_scratch_bytes", (n, rows.dim, cols), G.device)
+    aligned = 1 if (ld * G.element_size()) % 16 == 0 and G.data_ptr() % 16 == 0 else 0
+    try:
+        scratch, need = _scratch("pspmm_rows8_mm_t_scratch_bytes", (n, rows.dim, cols, _DTYPES[G.dtype], aligned), G.device)
+    except torch.cuda.OutOfMemoryError:
+        if aligned:
+            raise
+        # without the copy of G on aligned rows
+        scratch, need = _scratch("pspmm_rows8_mm_t_scratch_bytes", (n, rows.dim, cols, _DTYPES[G.dtype], 1), G.device)
     rc = lib().pspmm_rows8_mm_t(rows.q.data_ptr(), rows.q.shape[1], rows.scales.data_ptr(), n, rows.dim, G.data_ptr(),
                                 _DTYPES[G.dtype], ld, cols, out.data_ptr(), out.stride(0), _ptr(scratch), need, _stream())
     if rc:

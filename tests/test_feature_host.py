@@ -155,11 +155,16 @@ def test_operands_on_two_gpus_are_refused():
 def test_rows8_product_entry_point_refuses(pspmm_lib):
     from paramspmm_ae_b200 import _lib
     need = ctypes.c_size_t(0)
-    assert pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(100000, 64, 16, ctypes.byref(need)) == 0 and need.value > 0
+    assert pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(100000, 64, 16, 0, 1, ctypes.byref(need)) == 0 and need.value > 0
     size = need.value
-    assert pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(0, 64, 16, ctypes.byref(need)) == 0 and need.value == 0
-    _arg(pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(-1, 64, 16, ctypes.byref(need)))
-    _arg(pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(1, 64, 16, None))
+    assert pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(0, 64, 16, 0, 1, ctypes.byref(need)) == 0 and need.value == 0
+    _arg(pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(-1, 64, 16, 0, 1, ctypes.byref(need)))
+    _arg(pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(1, 64, 16, 0, 1, None))
+    _arg(pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(1, 64, 16, 3, 1, ctypes.byref(need)))
+    assert pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(100000, 64, 17, 1, 1, ctypes.byref(need)) == 0
+    without = need.value
+    assert pspmm_lib.pspmm_rows8_mm_t_scratch_bytes(100000, 64, 17, 1, 0, ctypes.byref(need)) == 0
+    assert need.value == without + 100000 * 24 * 2
 
     def mm(q=ONE, pitch=64, s=ONE, n=100000, dim=64, G=ONE, t=0, ld=16, cols=16, C=ONE, ldc=16, scratch=ONE, size=size):
         return pspmm_lib.pspmm_rows8_mm_t(q, pitch, s, n, dim, G, t, ld, cols, C, ldc, scratch, size, NULL)

@@ -54,6 +54,32 @@ def test_whole_numbers(dtype, dim, cols, n):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols,ld", [(47, 47), (1, 1), (2, 2), (7, 9), (33, 50), (130, 131), (64, 65)])
+@pytest.mark.parametrize("n", [1, 33, 1000, 10007])
+@pytest.mark.parametrize("at", [0, 1, 3])
+def test_unaligned_rows_without_room_for_a_copy(dtype, cols, ld, n, at):
+    """The C call with the scratch that it requires and no more; ``at``: where the first row begins."""
+    from paramspmm_ae_b200 import _lib
+    rows = held(n, 150, n + cols, exact=True)
+    store = torch.full((n * ld + 8,), float("nan"), dtype=dtype, device="cuda")
+    G = store[at:at + n * ld].view(n, ld)[:, :cols]
+    G.copy_(torch.randint(-4, 5, (n, cols), generator=torch.Generator().manual_seed(n)))
+    need = ctypes.c_size_t(0)
+    code = TYPES.index(dtype)
+    _lib.check(_lib.lib().pspmm_rows8_mm_t_scratch_bytes(n, 150, cols, code, 1, ctypes.byref(need)))
+    scratch = torch.empty(max(16, need.value), dtype=torch.uint8, device="cuda")
+    C = torch.full((150, cols), float("nan"), device="cuda")
+    _lib.check(_lib.lib().pspmm_rows8_mm_t(rows.q.data_ptr(), rows.q.shape[1], rows.scales.data_ptr(), n, 150, G.data_ptr(), code, ld,
+                                           cols, C.data_ptr(), cols, scratch.data_ptr(), need.value,
+                                           torch.cuda.current_stream().cuda_stream))
+    want = values(rows).t() @ G.double()
+    assert torch.equal(C.double(), want)
+    from paramspmm_ae_b200 import feature_ops as fo
+    if cols > 1:
+        assert torch.equal(fo.rows8_mm_t(rows, G).double(), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim,cols,n", [(1, 1, 5), (47, 8, 300), (100, 47, 2001), (256, 256, 9000), (500, 16, 19717), (1024, 1024, 3000),
                                         (64, 300, 100003), (1760, 103, 1501)])
 def test_real_values(dtype, dim, cols, n):
@@ -176,7 +202,7 @@ q, s, G = torch.ones(400, 64, dtype=torch.int8, device="cuda"), torch.ones(400, 
 rows = fo.Rows8(q, s, 64)
 assert (fo.rows8_mm_t(rows, G) == 400).all() and fo.rows8_mm_status() == 0
 need = ctypes.c_size_t(0)
-_lib.check(lib.pspmm_rows8_mm_t_scratch_bytes(400, 64, 32, ctypes.byref(need)))
+_lib.check(lib.pspmm_rows8_mm_t_scratch_bytes(400, 64, 32, 0, 1, ctypes.byref(need)))
 scratch = torch.zeros(max(need.value, 16), dtype=torch.uint8, device="cuda")
 C = torch.zeros(64, 32, device="cuda")
 _lib.check(lib.pspmm_rows8_mm_t_stalled(q.data_ptr(), 64, s.data_ptr(), 400, 64, G.data_ptr(), 0, 32, 32, C.data_ptr(), 32,
