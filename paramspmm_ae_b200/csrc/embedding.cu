@@ -3,12 +3,13 @@
 //
 // Lookup: a gather, bound by HBM (each row of the table once if ids repeat close together, each row of `out`).
 //
-// Gradient: the ids are sorted with their positions (stable, so that a row's sum has one order whatever the timing), and every
-// row of the table is then written once, zeros included, by one lane group that gathers the rows of G in the order of their
-// positions.  Ids that occur more than `run` times are cut into chunks of `run` sorted positions, whose sums are left in scratch and
-// added up by a dependent launch: no atomics on values, and the hottest id does not hold the launch up.
-// Up to RANK_MAX ids are sorted by counting, one launch; more by least-significant-digit passes of 8 bits (as many as the table's
-// size needs), three launches each.
+// Gradient: the ids are sorted with their positions (stable, so that a row's sum has one order whatever the timing).  Lane groups then
+// take equal chunks of sorted positions, gather the rows of G in that order and store a row of dT where an id's run of positions ends.
+// Runs that cross the border of a chunk leave their pieces in scratch, which a dependent launch adds in order: no atomics
+// on values, and the hottest id does not hold the launch up.  The rows that no id names are zeroed, with all others, by CTAs of the
+// sorting kernels, which leave the memory system idle.
+// Up to RANK_MAX ids are sorted by counting, one launch; more by least-significant-digit passes of up to 8 bits, as many as the
+// table's size needs, one or two launches each: a pass counts the digits of the next one while it places its keys.
 // Ids outside the table: NaN rows in the lookup, nothing in the gradient, and pspmm_embedding_status tells.
 #include "feature_types.cuh"
 
@@ -20,13 +21,14 @@ __device__ unsigned g_embedding_status;
 constexpr int RANK_MAX = 2048;
 constexpr int TILE_THREADS = 256, TILE_KEYS = 8, TILE = TILE_THREADS * TILE_KEYS;  // keys of a CTA in a digit pass
 constexpr int WARPS = TILE_THREADS / 32;
-constexpr int MOST_TOKENS = 256;  // rows of the table that a CTA writes
+constexpr int SCAN_TILES = 32;
+constexpr int HOT = 64;  // chunks from which on a run's pieces are added by a CTA
 
 struct LookupArgs {
     const void *ids, *table;
     void *out;
     int64_t n, n_rows, ld_table, ld_out;
-    int32_t ids64, vecs, lanes;  // vectors per row, lanes that share a row
+    int32_t ids64, cols;
     float scale;
 };
 
@@ -36,31 +38,54 @@ struct Ids {
     int32_t ids64;
 };
 
+// Memory that the sorting kernels zero beside their work: a share of it each.
+struct Fill {
+    char *p;
+    int64_t bytes;
+    int32_t share, shares, ctas;
+};
+
+// Sorted and unsorted ids are pairs: sort key in x, position in y.
 struct SortArgs {
     Ids in;
-    const uint32_t *key_in;  // null: the first pass, from `in`
-    const uint32_t *pos_in;
-    uint32_t *key_out, *pos_out;
-    uint32_t *counts;  // [256][tiles], turned into each tile's first place inside its digit
-    uint32_t *totals;  // [256]
+    const uint2 *from;  // null: the first pass, from `in`
+    uint2 *to;
+    uint32_t *counts;   // keys of each digit and tile; where scanned, each tile's first place inside its digit
+    uint32_t *totals;   // [256] of a scanned pass; null: the tiles add up the counts before them on their own
+    uint32_t *next;     // counts of the next pass, added up while this one's keys are placed; null: there is none
     int32_t tiles, shift;
+    int32_t passes, bits, mask;  // of a digit
+    int32_t work;       // CTAs that sort; those behind them fill
+    Fill fill;
 };
 
 struct GradArgs {
-    const uint32_t *keys, *pos;  // sorted
+    const uint2 *ids;   // sorted
     const void *grad;
     void *out;
-    float *part;     // [chunks][2][cols]: the piece that begins before the chunk or with it, and the one that begins inside
+    float *part;        // [chunks][2][cols]: the piece that begins with the chunk, and the one that begins inside and goes on
     int64_t n, n_rows, ld_grad, ld_out;
-    int64_t units;   // chunks * slices
-    int32_t chunk_ctas;  // the first CTAs of the launch take chunks
-    int32_t run, vecs, lanes, slices, tokens, cols;
+    int64_t units;      // chunks * slices
+    int32_t run, vecs, slices, cols;
+    int32_t hot_ctas;   // combine: the first CTAs take runs of more than HOT chunks
     float scale;
 };
 
 __device__ __forceinline__ int64_t load_id(const void *ids, int ids64, int64_t i)
 {
     return ids64 ? static_cast<const int64_t *>(ids)[i] : (int64_t)static_cast<const int32_t *>(ids)[i];
+}
+// A store that does not displace what the caches hold.
+template <typename T, int VW> __device__ __forceinline__ void store_past(T *p, const Vec<T, VW> &v)
+{
+    if constexpr (sizeof(v) == 16)
+        __stcs(reinterpret_cast<uint4 *>(p), *reinterpret_cast<const uint4 *>(&v));
+    else if constexpr (sizeof(v) == 8)
+        __stcs(reinterpret_cast<uint2 *>(p), *reinterpret_cast<const uint2 *>(&v));
+    else if constexpr (sizeof(v) == 4)
+        __stcs(reinterpret_cast<uint32_t *>(p), *reinterpret_cast<const uint32_t *>(&v));
+    else
+        __stcs(reinterpret_cast<unsigned short *>(p), *reinterpret_cast<const unsigned short *>(&v));
 }
 // Sort key of position i: its id, or n_rows (the last key) where no row takes the gradient.
 __device__ __forceinline__ uint32_t load_key(const Ids &a, int64_t i)
@@ -72,56 +97,93 @@ __device__ __forceinline__ uint32_t load_key(const Ids &a, int64_t i)
     return (uint32_t)(in && id != a.padding ? id : a.n_rows);
 }
 
-// `lanes` lanes share a row, ROWS rows of a lane group are in flight together.
-template <typename T, int VW, int ROWS>
+// L lanes share a row; a lane group takes ROWS neighbouring rows of the output and has them in flight together.  A warp's ids are looked at
+// by a lane each (by all of them: 52 instructions per 32 values of rows of 47, 24 us against 17).  Stored past the caches' order, so that the
+// table's rows stay.
+template <typename T, int VW, int L, int ROWS>
 __global__ void __launch_bounds__(256) lookup_kernel(const LookupArgs a)
 {
-    const int gl = threadIdx.x % a.lanes;
-    const int64_t groups = (int64_t)gridDim.x * (256 / a.lanes);
-    const int64_t group = (int64_t)blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
+    typedef Vec<T, VW> V;
+    constexpr int PER_WARP = 32 / L * ROWS;
+    static_assert(PER_WARP <= 32, "a lane per row");
+    const int lane = threadIdx.x % 32;
+    const int64_t first = ((int64_t)blockIdx.x * 8 + threadIdx.x / 32) * PER_WARP;
+    if (first >= a.n)
+        return;
+    int64_t at = -1;
+    if (lane < PER_WARP && first + lane < a.n) {
+        const int64_t id = load_id(a.ids, a.ids64, first + lane);
+        if (id >= 0 && id < a.n_rows)
+            at = id * a.ld_table;
+        else
+            g_embedding_status = 1;
+    }
+    int64_t from[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+        from[r] = __shfl_sync(PSPMM_FULL_MASK, at, lane / L * ROWS + r);
+    const int64_t i0 = first + lane / L * ROWS;
+    const int rows = a.n - i0 < ROWS ? (int)(a.n - i0) : ROWS;
     const float nan = __int_as_float(0x7fc00000);
-    for (int64_t i0 = group; i0 < a.n; i0 += groups * ROWS) {
-        int64_t id[ROWS];
+    const T *table = static_cast<const T *>(a.table);
+    T *out = static_cast<T *>(a.out) + i0 * a.ld_out;
+    for (int c = lane % L * VW; c < a.cols; c += L * VW) {
+        V f[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            const int64_t i = i0 + r * groups;
-            id[r] = i < a.n ? load_id(a.ids, a.ids64, i) : -1;
-            if (i < a.n && (id[r] < 0 || id[r] >= a.n_rows)) {
-                id[r] = -1;
-                g_embedding_status = 1;
-            }
-        }
-        for (int v = gl; v < a.vecs; v += a.lanes) {
-            float f[ROWS][VW];
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r) {
-                if (id[r] >= 0) {
-                    load_vec<T, VW>(f[r], static_cast<const T *>(a.table) + id[r] * a.ld_table + (int64_t)v * VW);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VW; ++j)
-                        f[r][j] = nan;
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r) {
+            if (from[r] >= 0) {
+                f[r] = *reinterpret_cast<const V *>(table + from[r] + c);
+            } else {
 #pragma unroll
                 for (int j = 0; j < VW; ++j)
-                    f[r][j] *= a.scale;
-                const int64_t i = i0 + r * groups;
-                if (i < a.n)
-                    store_vec<T, VW>(static_cast<T *>(a.out) + i * a.ld_out + (int64_t)v * VW, f[r]);
+                    f[r].v[j] = from_float<T>(nan);
             }
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+            for (int j = 0; j < VW; ++j)
+                f[r].v[j] = from_float<T>(to_float(f[r].v[j]) * a.scale);
+            if (r < rows)
+                store_past(out + r * a.ld_out + c, f[r]);
         }
     }
 }
 
 // ---- sorting -------------------------------------------------------------------------------------------------------
 
+// A share of the memory, cut at 16 bytes, by the CTAs from `work` on.
+__device__ __forceinline__ void fill_zeros(const Fill &f, int cta)
+{
+    const int64_t lead = min((int64_t)(-(uintptr_t)f.p & 15), f.bytes), whole = (f.bytes - lead) / 16;
+    uint4 *p = reinterpret_cast<uint4 *>(f.p + lead);
+    const int64_t from = whole * f.share / f.shares, to = whole * (f.share + 1) / f.shares;
+    for (int64_t i = from + (int64_t)cta * 256 + threadIdx.x; i < to; i += (int64_t)f.ctas * 256)
+        p[i] = make_uint4(0, 0, 0, 0);
+    if (f.share == 0 && cta == 0) {  // the ends (elements of 2 or 4 bytes)
+        uint16_t *q = reinterpret_cast<uint16_t *>(f.p);
+        for (int64_t i = threadIdx.x; i < lead / 2; i += 256)
+            q[i] = 0;
+        for (int64_t i = (lead + whole * 16) / 2 + threadIdx.x; i < f.bytes / 2; i += 256)
+            q[i] = 0;
+    }
+}
+
+// Counts lie by tile where the tiles read them all, else by digit.
+__device__ __forceinline__ int64_t count_at(const SortArgs &a, int64_t tile, uint32_t digit)
+{
+    return a.totals ? digit * (int64_t)a.tiles + tile : tile * 256 + digit;
+}
+
 // Few ids: the place of a key is the number of smaller ones and of equal ones before it; a warp counts for one key.
 __global__ void __launch_bounds__(256) rank_kernel(const SortArgs a)
 {
     __shared__ uint32_t keys[RANK_MAX];
+    pdl_launch_dependents();
+    if ((int)blockIdx.x >= a.work) {
+        fill_zeros(a.fill, blockIdx.x - a.work);
+        return;
+    }
     const int n = (int)a.in.n, lane = threadIdx.x % 32;
     for (int i = threadIdx.x; i < n; i += 256)
         keys[i] = load_key(a.in, i);
@@ -134,29 +196,40 @@ __global__ void __launch_bounds__(256) rank_kernel(const SortArgs a)
     for (int j = lane; j < n; j += 32)
         before += keys[j] < key || (keys[j] == key && j < i);
     before = __reduce_add_sync(PSPMM_FULL_MASK, before);
-    if (lane == 0) {
-        a.key_out[before] = key;
-        a.pos_out[before] = (uint32_t)i;
-    }
+    if (lane == 0)
+        a.to[before] = make_uint2(key, (uint32_t)i);
 }
 
-__device__ __forceinline__ uint32_t sort_key(const SortArgs &a, int64_t i)
+__device__ __forceinline__ uint2 sort_pair(const SortArgs &a, int64_t i)
 {
-    return a.key_in ? a.key_in[i] : load_key(a.in, i);
+    return a.from ? a.from[i] : make_uint2(load_key(a.in, i), (uint32_t)i);
 }
 
+// Of the first pass; the others are counted by the pass before.
 __global__ void __launch_bounds__(TILE_THREADS) digit_count_kernel(const SortArgs a)
 {
     __shared__ uint32_t bins[256];
+    pdl_launch_dependents();
+    if ((int)blockIdx.x >= a.work) {
+        fill_zeros(a.fill, blockIdx.x - a.work);
+        return;
+    }
     bins[threadIdx.x] = 0;
+    for (int p = 1; p < a.passes; ++p)
+        a.counts[((int64_t)p * a.tiles + blockIdx.x) * 256 + threadIdx.x] = 0;
     __syncthreads();
+    uint32_t key[TILE_KEYS];
+#pragma unroll
     for (int k = 0; k < TILE_KEYS; ++k) {
         const int64_t i = (int64_t)blockIdx.x * TILE + k * TILE_THREADS + threadIdx.x;
-        if (i < a.in.n)
-            atomicAdd(&bins[sort_key(a, i) >> a.shift & 255], 1u);
+        key[k] = i < a.in.n ? load_key(a.in, i) : 0;
     }
+#pragma unroll
+    for (int k = 0; k < TILE_KEYS; ++k)
+        if ((int64_t)blockIdx.x * TILE + k * TILE_THREADS + threadIdx.x < a.in.n)
+            atomicAdd(&bins[key[k] >> a.shift & a.mask], 1u);
     __syncthreads();
-    a.counts[(int64_t)threadIdx.x * a.tiles + blockIdx.x] = bins[threadIdx.x];
+    a.counts[count_at(a, blockIdx.x, threadIdx.x)] = bins[threadIdx.x];
 }
 
 // Sum over the threads before this one, in a CTA of 256; `warps` is scratch of 8.
@@ -188,6 +261,12 @@ __device__ __forceinline__ uint32_t exclusive_256(uint32_t v, uint32_t *warps, u
 __global__ void __launch_bounds__(256) digit_scan_kernel(const SortArgs a)
 {
     __shared__ uint32_t warps[8];
+    pdl_launch_dependents();
+    if ((int)blockIdx.x >= a.work) {
+        fill_zeros(a.fill, blockIdx.x - a.work);
+        return;
+    }
+    pdl_wait();
     uint32_t *c = a.counts + (int64_t)blockIdx.x * a.tiles;
     uint32_t carry = 0;
     for (int t0 = 0; t0 < a.tiles; t0 += 256) {
@@ -204,31 +283,47 @@ __global__ void __launch_bounds__(256) digit_scan_kernel(const SortArgs a)
 }
 
 // Stable: a warp takes 256 neighbouring keys, 32 at a time; equal digits among the 32 find one another by a match, and a
-// count per warp and digit carries on from one 32 to the next.
+// count per warp and digit carries on from one 32 to the next.  The tile is put in order in shared memory, so that equal digits leave
+// side by side.
 __global__ void __launch_bounds__(TILE_THREADS) digit_scatter_kernel(const SortArgs a)
 {
     __shared__ uint32_t seen[WARPS][256];
-    __shared__ uint32_t first[256];
+    __shared__ uint32_t away[256];  // from a key's place in the tile to its place among all
     __shared__ uint32_t warps[8];
+    __shared__ uint2 tile[TILE];
+    pdl_launch_dependents();
+    if ((int)blockIdx.x >= a.work) {
+        fill_zeros(a.fill, blockIdx.x - a.work);
+        return;
+    }
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    uint32_t total;
-    first[threadIdx.x] = exclusive_256(a.totals[threadIdx.x], warps, total) +
-                         a.counts[(int64_t)threadIdx.x * a.tiles + blockIdx.x];
     for (int w = 0; w < WARPS; ++w)
         seen[w][threadIdx.x] = 0;
-    __syncthreads();
-    uint32_t key[TILE_KEYS], pos[TILE_KEYS], rank[TILE_KEYS];
+    pdl_wait();
+    uint2 pair[TILE_KEYS];
+    uint32_t rank[TILE_KEYS];
     const int64_t i0 = (int64_t)blockIdx.x * TILE + warp * (32 * TILE_KEYS) + lane;
 #pragma unroll
-    for (int k = 0; k < TILE_KEYS; ++k) {
-        const int64_t i = i0 + k * 32;
-        key[k] = i < a.in.n ? sort_key(a, i) : 0xffffffffu;
-        pos[k] = i < a.in.n ? (a.pos_in ? a.pos_in[i] : (uint32_t)i) : 0;
+    for (int k = 0; k < TILE_KEYS; ++k)
+        if (i0 + k * 32 < a.in.n)
+            pair[k] = sort_pair(a, i0 + k * 32);
+    uint32_t total, all = 0, earlier = 0;  // keys of this thread's digit: in all tiles, in those before this one
+    if (a.totals) {
+        all = a.totals[threadIdx.x];
+        earlier = a.counts[count_at(a, blockIdx.x, threadIdx.x)];
+    } else {
+#pragma unroll 16
+        for (int t = 0; t < a.tiles; ++t) {
+            const uint32_t c = a.counts[t * 256 + threadIdx.x];
+            all += c;
+            earlier += t < (int)blockIdx.x ? c : 0;
+        }
     }
+    const uint32_t first = exclusive_256(all, warps, total) + earlier;
 #pragma unroll
     for (int k = 0; k < TILE_KEYS; ++k) {
         const bool in = i0 + k * 32 < a.in.n;
-        const uint32_t d = in ? key[k] >> a.shift & 255 : 256;  // (lanes beyond the end match one another only)
+        const uint32_t d = in ? pair[k].x >> a.shift & a.mask : 256;  // (lanes beyond the end match one another only)
         const uint32_t same = __match_any_sync(PSPMM_FULL_MASK, d);
         const uint32_t below = __popc(same & ((1u << lane) - 1));
         rank[k] = in ? seen[warp][d] + below : 0;
@@ -238,7 +333,11 @@ __global__ void __launch_bounds__(TILE_THREADS) digit_scatter_kernel(const SortA
         __syncwarp();
     }
     __syncthreads();
-    uint32_t before = first[threadIdx.x];
+    uint32_t mine = 0;
+    for (int w = 0; w < WARPS; ++w)
+        mine += seen[w][threadIdx.x];
+    uint32_t before = exclusive_256(mine, warps, total);
+    away[threadIdx.x] = first - before;
     for (int w = 0; w < WARPS; ++w) {
         const uint32_t c = seen[w][threadIdx.x];
         seen[w][threadIdx.x] = before;
@@ -247,21 +346,35 @@ __global__ void __launch_bounds__(TILE_THREADS) digit_scatter_kernel(const SortA
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < TILE_KEYS; ++k)
-        if (i0 + k * 32 < a.in.n) {
-            const uint32_t to = seen[warp][key[k] >> a.shift & 255] + rank[k];
-            a.key_out[to] = key[k];
-            a.pos_out[to] = pos[k];
+        if (i0 + k * 32 < a.in.n)
+            tile[seen[warp][pair[k].x >> a.shift & a.mask] + rank[k]] = pair[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < TILE_KEYS; ++k) {
+        const uint32_t j = k * TILE_THREADS + threadIdx.x;
+        uint32_t place = 0xffffffffu;
+        if (j < total) {
+            const uint2 v = tile[j];
+            const uint32_t to = away[v.x >> a.shift & a.mask] + j;
+            a.to[to] = v;
+            place = (uint32_t)count_at(a, to / TILE, v.x >> (a.shift + a.bits) & a.mask);
         }
+        if (a.next) {  // (hot ids and short last digits would have the lanes add to one place in turn)
+            const uint32_t same = __match_any_sync(PSPMM_FULL_MASK, place);
+            if (place != 0xffffffffu && (same & ((1u << lane) - 1)) == 0)
+                atomicAdd(&a.next[place], (uint32_t)__popc(same));
+        }
+    }
 }
 
 // ---- sums ----------------------------------------------------------------------------------------------------------
 
 // First position in [lo, hi) whose key is not below `key` (hi: none).
-__device__ __forceinline__ int64_t lower_bound(const uint32_t *keys, uint32_t key, int64_t lo, int64_t hi)
+__device__ __forceinline__ int64_t lower_bound(const uint2 *ids, uint32_t key, int64_t lo, int64_t hi)
 {
     while (lo < hi) {
         const int64_t mid = (lo + hi) >> 1;
-        if (keys[mid] < key)
+        if (ids[mid].x < key)
             lo = mid + 1;
         else
             hi = mid;
@@ -269,15 +382,15 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t *keys, uint32_t ke
     return lo;
 }
 
-// The same over all keys by a whole warp, 32 probes a step.
-__device__ __forceinline__ int64_t warp_lower_bound(const uint32_t *keys, uint32_t key, int64_t n)
+// The same over [lo, n) by a whole warp, 32 probes a step.
+__device__ __forceinline__ int64_t warp_lower_bound(const uint2 *ids, uint32_t key, int64_t lo, int64_t n)
 {
     const int lane = threadIdx.x % 32;
-    int64_t lo = 0, hi = n;  // the answer lies in [lo, hi]
+    int64_t hi = n;  // the answer lies in [lo, hi]
     while (hi - lo > 32) {
         const int64_t step = (hi - lo + 31) / 32;
         const int64_t at = lo + lane * step;
-        const bool below = at < hi && keys[at] < key;
+        const bool below = at < hi && ids[at].x < key;
         const int c = __popc(__ballot_sync(PSPMM_FULL_MASK, below));
         if (c == 0)
             return lo;
@@ -285,195 +398,188 @@ __device__ __forceinline__ int64_t warp_lower_bound(const uint32_t *keys, uint32
         lo = from + 1;
         hi = from + step < hi ? from + step : hi;
     }
-    const bool below = lo + lane < hi && keys[lo + lane] < key;
+    const bool below = lo + lane < hi && ids[lo + lane].x < key;
     return lo + __popc(__ballot_sync(PSPMM_FULL_MASK, below));
 }
 
-// Sum of the rows of G at sorted positions [p, e), one vector of columns.
-template <typename T, int VW>
-__device__ __forceinline__ void gather_sum(float (&acc)[VW], const GradArgs &a, int64_t p, int64_t e, int v)
+// A group of L lanes per chunk and slice of columns, a vector per lane, U rows in flight; a lane looks at a position, and the places of the
+// rows and of the runs' beginnings go round by shuffles and a ballot.  (Two or four vectors per lane and row: fewer groups and fewer rows
+// each; 32,768 rows of 1,024 bf16 31 us against 17.)
+template <typename T, int VW, int L>
+__global__ void __launch_bounds__(256, 3) grad_kernel(const GradArgs a)
 {
-    constexpr int U = 4;
-    const T *g = static_cast<const T *>(a.grad) + (int64_t)v * VW;
-#pragma unroll
-    for (int j = 0; j < VW; ++j)
-        acc[j] = 0.f;
-    for (; p + U <= e; p += U) {
-        float f[U][VW];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            load_vec<T, VW>(f[u], g + (int64_t)a.pos[p + u] * a.ld_grad);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < VW; ++j)
-                acc[j] += f[u][j];
-    }
-    for (; p < e; ++p) {
-        float f[VW];
-        load_vec<T, VW>(f, g + (int64_t)a.pos[p] * a.ld_grad);
-#pragma unroll
-        for (int j = 0; j < VW; ++j)
-            acc[j] += f[j];
-    }
-}
-
-template <typename T, int VW>
-__device__ __forceinline__ void chunk_part(const GradArgs &a, int64_t chunk, int slot, int64_t p, int64_t e, int v)
-{
-    float acc[VW];
-    gather_sum<T, VW>(acc, a, p, e, v);
-    float *part = a.part + (chunk * 2 + slot) * a.cols + (int64_t)v * VW;
-#pragma unroll
-    for (int j = 0; j < VW; ++j)
-        part[j] = acc[j];
-}
-
-// Whether the id at position p, the first of its run, occurs more than `run` times.
-__device__ __forceinline__ bool is_long(const GradArgs &a, int64_t p)
-{
-    return p + a.run < a.n && a.keys[p + a.run] == a.keys[p];
-}
-
-template <typename T, int VW>
-__global__ void __launch_bounds__(256) grad_kernel(const GradArgs a)
-{
-    __shared__ int64_t start[MOST_TOKENS + 1];
-    __shared__ int64_t range[2];
+    constexpr int U = L < 8 ? L : sizeof(T) * VW <= 4 && L >= 16 ? 16 : 8;
+    typedef Vec<T, VW> V;
     pdl_launch_dependents();
-    pdl_wait();
-    const int gl = threadIdx.x % a.lanes, group = threadIdx.x / a.lanes, groups = 256 / a.lanes;
-    if ((int)blockIdx.x < a.chunk_ctas) {  // a lane group per chunk and slice of columns
-        const int64_t unit = (int64_t)blockIdx.x * groups + group;
-        if (unit >= a.units)
-            return;
-        const int64_t chunk = unit / a.slices;
-        const int v = (int)(unit % a.slices) * a.lanes + gl;
-        if (v >= a.vecs)
-            return;
-        const int64_t begin = chunk * a.run, end = begin + a.run < a.n ? begin + a.run : a.n;
-        const uint32_t head = a.keys[begin], tail = a.keys[end - 1];
-        if (head < a.n_rows) {
-            const int64_t from = begin > a.run ? begin - a.run : 0;
-            const int64_t s = lower_bound(a.keys, head, from, begin);
-            // (a run that reaches `run` places back is long; so is one whose first position says so)
-            if ((s == from && begin - from == a.run) || is_long(a, s))
-                chunk_part<T, VW>(a, chunk, 0, begin, lower_bound(a.keys, head + 1, begin, end), v);
-        }
-        if (tail != head && tail < a.n_rows) {
-            const int64_t s = lower_bound(a.keys, tail, begin, end);
-            if (is_long(a, s))
-                chunk_part<T, VW>(a, chunk, 1, s, end, v);
-        }
+    const int64_t unit = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (unit >= a.units)
         return;
-    }
-    const int64_t t0 = (int64_t)(blockIdx.x - a.chunk_ctas) * a.tokens;
-    const int tokens = a.n_rows - t0 < a.tokens ? (int)(a.n_rows - t0) : a.tokens;
-    if (threadIdx.x < 64) {
-        const int64_t at = warp_lower_bound(a.keys, (uint32_t)(t0 + (threadIdx.x < 32 ? 0 : tokens)), a.n);
-        if (threadIdx.x % 32 == 0)
-            range[threadIdx.x / 32] = at;
-    }
-    __syncthreads();
-    for (int t = threadIdx.x; t <= tokens; t += 256)
-        start[t] = lower_bound(a.keys, (uint32_t)(t0 + t), range[0], range[1]);
-    __syncthreads();
-    for (int t = group; t < tokens; t += groups) {
-        const int64_t s = start[t], e = start[t + 1];
-        if (e - s > a.run)
-            continue;  // cut into chunks
-        T *out = static_cast<T *>(a.out) + (t0 + t) * a.ld_out;
-        for (int v = gl; v < a.vecs; v += a.lanes) {
-            float acc[VW];
-            gather_sum<T, VW>(acc, a, s, e, v);
+    const int lane = threadIdx.x % 32, group = lane / L * L, look = lane % U;
+    const uint32_t mask = L == 32 ? PSPMM_FULL_MASK : ((1u << L) - 1) << group;
+    const int64_t chunk = unit / a.slices;
+    const int v = (int)(unit % a.slices) * L + lane % L;
+    const int64_t begin = chunk * a.run, end = begin + a.run < a.n ? begin + a.run : a.n;
+    // (lanes beyond the row's vectors load the last one again)
+    const T *grad = static_cast<const T *>(a.grad) + (int64_t)min(v, a.vecs - 1) * VW;
+    const bool mine = v < a.vecs;
+    float acc[VW] = {};
+    pdl_wait();
+    uint32_t key = a.ids[begin].x;
+    const bool goes_on = end < a.n && a.ids[end - 1].x == a.ids[end].x;  // the last run, behind the chunk
+    bool whole = begin == 0 || a.ids[begin - 1].x != key, head = true;   // of the run at hand: begins here; with the chunk
+    auto finish = [&](bool ends) {
+        if (key >= a.n_rows || !mine)
+            return;
+        if (whole && ends) {
 #pragma unroll
             for (int j = 0; j < VW; ++j)
                 acc[j] *= a.scale;
-            store_vec<T, VW>(out + (int64_t)v * VW, acc);
+            store_vec<T, VW>(static_cast<T *>(a.out) + (int64_t)key * a.ld_out + (int64_t)v * VW, acc);
+        } else {
+            float *part = a.part + (chunk * 2 + (head ? 0 : 1)) * a.cols + (int64_t)v * VW;
+#pragma unroll
+            for (int j = 0; j < VW; ++j)
+                part[j] = acc[j];
+        }
+    };
+    for (int64_t p = begin; p < end; p += U) {
+        const uint2 id = a.ids[p + look < end ? p + look : end - 1];
+        const uint32_t before = __shfl_up_sync(mask, id.x, 1);
+        const uint32_t begins = __ballot_sync(mask, id.x != (look == 0 ? key : before)) >> group;
+        const int64_t at = (int64_t)id.y * a.ld_grad;
+        V f[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            f[u] = *reinterpret_cast<const V *>(grad + __shfl_sync(mask, at, group + u));
+        const int here = end - p < U ? (int)(end - p) : U;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= here)
+                break;
+            if (begins >> u & 1) {
+                finish(true);
+                key = __shfl_sync(mask, id.x, group + u);
+                whole = true;
+                head = false;
+#pragma unroll
+                for (int j = 0; j < VW; ++j)
+                    acc[j] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < VW; ++j)
+                acc[j] += to_float(f[u].v[j]);
         }
     }
+    finish(!goes_on);
 }
 
-// The chunks' sums of each long run, added in order: a CTA looks at 256 chunks for runs that begin there.
+// The pieces of each run that crosses chunks, added in order.  A warp per chunk and 128 columns looks for the run that begins in the
+// chunk and goes on; one of more than HOT chunks is left to a CTA per HOT chunks and 16 columns, sixteen shares of the pieces each.
 template <typename T>
 __global__ void __launch_bounds__(256) combine_kernel(const GradArgs a)
 {
-    __shared__ int64_t begins[256];
-    __shared__ int64_t ends;
-    __shared__ int found;
-    __shared__ float sums[256];
-    if (threadIdx.x == 0)
-        found = 0;
-    __syncthreads();
-    pdl_wait();
+    __shared__ float sums[16][17];
     const int64_t chunks = (a.n + a.run - 1) / a.run;
-    const int64_t chunk = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (chunk < chunks) {
-        // A run that begins in a chunk and is long reaches the chunk's end.
-        const int64_t begin = chunk * a.run, end = begin + a.run < a.n ? begin + a.run : a.n;
-        const uint32_t tail = a.keys[end - 1];
-        if (tail < a.n_rows) {
-            const int64_t s = lower_bound(a.keys, tail, begin, end);
-            if ((s > begin || s == 0 || a.keys[s - 1] != tail) && is_long(a, s))
-                begins[atomicAdd(&found, 1)] = s;
-        }
-    }
-    __syncthreads();
-    // Threads: `wide` columns side by side, 256 / wide shares of a run's chunks.
-    int wide = 256;
-    while (wide / 2 >= a.cols)
-        wide /= 2;
-    const int shares = 256 / wide, share = threadIdx.x / wide;
-    for (int f = 0; f < found; ++f) {
-        const int64_t s = begins[f];
-        const uint32_t key = a.keys[s];
-        if (threadIdx.x < 32) {
-            const int64_t e = warp_lower_bound(a.keys, key + 1, a.n);
-            if (threadIdx.x == 0)
-                ends = e;
-        }
-        __syncthreads();
-        const int64_t c0 = s / a.run, c1 = (ends - 1) / a.run;
-        const int64_t per = (c1 - c0 + shares) / shares;  // chunks of a share, of c1 - c0 + 1
+    const uint2 *ids = a.ids;
+    pdl_wait();
+    if ((int)blockIdx.x < a.hot_ctas) {
+        const int tiles = (a.cols + 15) / 16;
+        const int64_t first = (int64_t)(blockIdx.x / tiles) * HOT * a.run, next = first + (int64_t)HOT * a.run;
+        if (next >= a.n)
+            return;
+        const uint32_t key = ids[next].x;
+        if (key >= a.n_rows || ids[next - 1].x != key)
+            return;
+        const int64_t s = lower_bound(ids, key, first, next);
+        if (s == first && first > 0 && ids[first - 1].x == key)
+            return;
+        const int64_t c0 = s / a.run;
+        if ((c0 + HOT) * a.run >= a.n || ids[(c0 + HOT) * a.run].x != key)
+            return;
+        const int64_t c1 = (warp_lower_bound(ids, key + 1, next, a.n) - 1) / a.run;
+        const int col = (int)(blockIdx.x % tiles) * 16 + threadIdx.x % 16, share = threadIdx.x / 16;
+        const int64_t per = (c1 - c0 + 16) / 16;
         const int64_t from = c0 + share * per, to = from + per <= c1 ? from + per : c1 + 1;
-        for (int col0 = 0; col0 < a.cols; col0 += wide) {
-            const int col = col0 + threadIdx.x % wide;
-            float sum = 0.f;
-            if (col < a.cols)
-                for (int64_t c = from; c < to; ++c)
-                    sum += a.part[(c * 2 + (c == c0 && s != c0 * a.run ? 1 : 0)) * a.cols + col];
-            sums[threadIdx.x] = sum;
-            __syncthreads();
-            if (share == 0 && col < a.cols) {
-                for (int i = 1; i < shares; ++i)
-                    sum += sums[i * wide + threadIdx.x];
-                static_cast<T *>(a.out)[(int64_t)key * a.ld_out + col] = from_float<T>(sum * a.scale);
-            }
-            __syncthreads();
+        float sum = 0.f;
+        if (col < a.cols) {
+            const int inside = s != c0 * a.run ? 1 : 0;
+#pragma unroll 8
+            for (int64_t c = from; c < to; ++c)
+                sum += a.part[(c * 2 + (c == c0 ? inside : 0)) * a.cols + col];
         }
+        sums[share][threadIdx.x % 16] = sum;
+        __syncthreads();
+        if (share == 0 && col < a.cols) {
+#pragma unroll
+            for (int i = 1; i < 16; ++i)
+                sum += sums[i][threadIdx.x];
+            static_cast<T *>(a.out)[(int64_t)key * a.ld_out + col] = from_float<T>(sum * a.scale);
+        }
+        return;
     }
+    const int tiles = (a.cols + 127) / 128, lane = threadIdx.x % 32;
+    const int64_t unit = (int64_t)(blockIdx.x - a.hot_ctas) * 8 + threadIdx.x / 32;
+    const int64_t chunk = unit / tiles;
+    if (chunk >= chunks)
+        return;
+    const int64_t begin = chunk * a.run, end = begin + a.run;
+    if (end >= a.n)
+        return;
+    const uint32_t key = ids[end].x;
+    if (key >= a.n_rows || ids[end - 1].x != key)
+        return;
+    const int64_t s = lower_bound(ids, key, begin, end);
+    if (s == begin && begin > 0 && ids[begin - 1].x == key)
+        return;
+    const int64_t far = (chunk + HOT) * a.run;
+    if (far < a.n && ids[far].x == key)
+        return;
+    const int64_t c1 = (lower_bound(ids, key + 1, end, far < a.n ? far : a.n) - 1) / a.run;
+    const int col = (int)(unit % tiles) * 128 + lane;
+    float sum[4] = {};
+    for (int64_t c0 = chunk; c0 <= c1; c0 += 4) {
+        float f[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t c = c0 + u;
+            const float *part = a.part + (c * 2 + (c == chunk && s != begin ? 1 : 0)) * a.cols + col;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                f[u][t] = c <= c1 && col + 32 * t < a.cols ? part[32 * t] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                sum[t] += f[u][t];
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+        if (col + 32 * t < a.cols)
+            static_cast<T *>(a.out)[(int64_t)key * a.ld_out + col + 32 * t] = from_float<T>(sum[t] * a.scale);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
 
-int lanes_for(int64_t vecs)
+template <typename T, int VW, int L> cudaError_t launch_lookup_lanes(const LookupArgs &a, cudaStream_t st)
 {
-    int l = 1;
-    while (l < 32 && l < vecs)
-        l *= 2;
-    return l;
+    constexpr int MOST = L < 8 ? L : 8;
+    const int64_t groups = 256 / L, ctas = (a.n + groups - 1) / groups;
+    // several rows per lane group where that still leaves every SM some CTAs
+    if (ctas >= MOST * 4 * (int64_t)pspmm_sm_count())
+        lookup_kernel<T, VW, L, MOST><<<(unsigned)((ctas + MOST - 1) / MOST), 256, 0, st>>>(a);
+    else
+        lookup_kernel<T, VW, L, 1><<<(unsigned)ctas, 256, 0, st>>>(a);
+    return cudaGetLastError();
 }
 
-template <typename T, int VW> cudaError_t launch_lookup(LookupArgs a, int32_t dim, cudaStream_t st)
+template <typename T, int VW> cudaError_t launch_lookup(const LookupArgs &a, int32_t dim, cudaStream_t st)
 {
-    a.vecs = dim / VW;
-    a.lanes = lanes_for(a.vecs);
-    const int64_t per_cta = 256 / a.lanes * 4;
-    int64_t ctas = (a.n + per_cta - 1) / per_cta;
-    const int64_t most = (int64_t)pspmm_sm_count() * 64;
-    ctas = ctas < most ? ctas : most;
-    lookup_kernel<T, VW, 4><<<(unsigned)ctas, 256, 0, st>>>(a);
-    return cudaGetLastError();
+    const int vecs = dim / VW;
+    return vecs <= 4    ? launch_lookup_lanes<T, VW, 4>(a, st)
+           : vecs <= 8  ? launch_lookup_lanes<T, VW, 8>(a, st)
+           : vecs <= 16 ? launch_lookup_lanes<T, VW, 16>(a, st)
+                        : launch_lookup_lanes<T, VW, 32>(a, st);
 }
 
 template <typename T> cudaError_t lookup_typed(const LookupArgs &a, int32_t dim, cudaStream_t st)
@@ -490,13 +596,13 @@ template <typename T> cudaError_t lookup_typed(const LookupArgs &a, int32_t dim,
     return launch_lookup<T, 1>(a, dim, st);
 }
 
-// Positions of a chunk: short ones spread a small call over the GPU, long ones leave fewer sums of a hot id to add up.
-int32_t run_for(int64_t n) { return n <= (1 << 16) ? 32 : n <= (1 << 18) ? 64 : n <= (1 << 20) ? 128 : 256; }
+// Positions of a chunk: short ones spread a small call over the GPU, long ones leave fewer pieces to add.
+int32_t run_for(int64_t n) { return n <= (1 << 12) ? 8 : n <= (1 << 16) ? 32 : n <= (1 << 20) ? 64 : 128; }
 
 size_t round_up(size_t v) { return (v + 255) / 256 * 256; }
 
 struct GradScratch {
-    size_t keys[2], pos[2], counts, totals, part, bytes;
+    size_t pairs[2], counts, totals, part, bytes;
 };
 GradScratch grad_scratch(int64_t n, int32_t dim)
 {
@@ -508,35 +614,36 @@ GradScratch grad_scratch(int64_t n, int32_t dim)
         at += round_up(bytes);
         return p;
     };
-    for (int i = 0; i < 2; ++i) {
-        s.keys[i] = take((size_t)n * 4);
-        s.pos[i] = take((size_t)n * 4);
-    }
-    s.counts = take(n > RANK_MAX ? tiles * 256 * 4 : 0);
-    s.totals = take(256 * 4);
+    for (int i = 0; i < 2; ++i)
+        s.pairs[i] = take(i == 0 || n > RANK_MAX ? (size_t)n * 8 : 0);
+    s.counts = take(n > RANK_MAX ? 4 * tiles * 256 * 4 : 0);  // of up to four passes
+    s.totals = take(n > RANK_MAX ? 256 * 4 : 0);
     const int64_t run = run_for(n);
     s.part = take(n > run ? (size_t)((n + run - 1) / run) * 2 * (size_t)dim * 4 : 0);
     s.bytes = at;
     return s;
 }
 
+template <typename T, int VW, int L> cudaError_t launch_grad_lanes(GradArgs a, cudaStream_t st)
+{
+    a.slices = (a.vecs + L - 1) / L;
+    const int64_t chunks = (a.n + a.run - 1) / a.run, per_cta = 256 / L;
+    a.units = chunks * a.slices;
+    cudaError_t e = launch_dependent(grad_kernel<T, VW, L>, dim3((unsigned)((a.units + per_cta - 1) / per_cta)), 256, 0, st, a);
+    if (e != cudaSuccess || chunks == 1)
+        return e;
+    a.hot_ctas = (int32_t)(chunks / HOT * ((a.cols + 15) / 16));
+    const int64_t warps = chunks * ((a.cols + 127) / 128);
+    return launch_dependent(combine_kernel<T>, dim3((unsigned)(a.hot_ctas + (warps + 7) / 8)), 256, 0, st, a);
+}
+
 template <typename T, int VW> cudaError_t launch_grad(GradArgs a, int32_t dim, cudaStream_t st)
 {
     a.vecs = dim / VW;
-    a.lanes = lanes_for(a.vecs);
-    a.slices = (a.vecs + a.lanes - 1) / a.lanes;
-    const int64_t chunks = a.n > a.run ? (a.n + a.run - 1) / a.run : 0;
-    a.units = chunks * a.slices;
-    const int64_t per_cta = 256 / a.lanes;
-    a.chunk_ctas = (int32_t)((a.units + per_cta - 1) / per_cta);
-    // about 32 KB of the table per CTA
-    int64_t tokens = (32 << 10) / ((int64_t)dim * sizeof(T));
-    a.tokens = (int32_t)(tokens < per_cta ? per_cta : tokens > MOST_TOKENS ? MOST_TOKENS : tokens);
-    const int64_t ctas = a.chunk_ctas + (a.n_rows + a.tokens - 1) / a.tokens;
-    cudaError_t e = launch_dependent(grad_kernel<T, VW>, dim3((unsigned)ctas), 256, 0, st, a);
-    if (e == cudaSuccess && chunks > 0)
-        e = launch_dependent(combine_kernel<T>, dim3((unsigned)((chunks + 255) / 256)), 256, 0, st, a);
-    return e;
+    return a.vecs <= 4    ? launch_grad_lanes<T, VW, 4>(a, st)
+           : a.vecs <= 8  ? launch_grad_lanes<T, VW, 8>(a, st)
+           : a.vecs <= 16 ? launch_grad_lanes<T, VW, 16>(a, st)
+                          : launch_grad_lanes<T, VW, 32>(a, st);
 }
 
 template <typename T> cudaError_t grad_typed(const GradArgs &a, int32_t dim, cudaStream_t st)
@@ -567,7 +674,9 @@ extern "C" int pspmm_embedding(const void *ids, int32_t ids64, int64_t n, const 
     const int B = elem_bytes(dtype);
     if (!ids || (!table && n_rows > 0) || !out || misaligned(ids, ids64 ? 8 : 4) || misaligned(table, B) || misaligned(out, B))
         return PSPMM_E_ARG;
-    const LookupArgs a = {ids, table, out, n, n_rows, ld_table, ld_out, ids64 != 0, 0, 0, scale};
+    if (dim > (1 << 24) || n > (int64_t)INT32_MAX * 8)
+        return PSPMM_E_RANGE;
+    const LookupArgs a = {ids, table, out, n, n_rows, ld_table, ld_out, ids64 != 0, dim, scale};
     cudaStream_t st = (cudaStream_t)stream;
     PSPMM_CUDA_TRY(dtype == PSPMM_F32    ? lookup_typed<float>(a, dim, st)
                    : dtype == PSPMM_BF16 ? lookup_typed<bf16>(a, dim, st)
@@ -594,9 +703,9 @@ extern "C" int pspmm_embedding_grad(const void *ids, int32_t ids64, int64_t n, c
     const int B = elem_bytes(dtype);
     if (!out || misaligned(out, B))
         return PSPMM_E_ARG;
-    // (CTAs take at least 8 rows of the table, at least a lane group per chunk and slice)
-    if (n > INT32_MAX - 65536 || n_rows > (int64_t)UINT32_MAX - 1 || dim > (1 << 24) ||
-        (n / run_for(n) + 1) * ((int64_t)dim / 32 + 1) + n_rows > INT32_MAX - 65536)
+    const int64_t chunks = n / run_for(n) + 1;  // (a warp per chunk and 32 columns at most, a CTA per HOT chunks and 16)
+    if (n > INT32_MAX - 65536 || n_rows > (int64_t)UINT32_MAX - 2 || dim > (1 << 24) ||
+        chunks * ((int64_t)dim / 32 + 1) + chunks / HOT * ((int64_t)dim / 16 + 1) > INT32_MAX - 65536)
         return PSPMM_E_RANGE;
     cudaStream_t st = (cudaStream_t)stream;
     if (n == 0) {
@@ -608,38 +717,52 @@ extern "C" int pspmm_embedding_grad(const void *ids, int32_t ids64, int64_t n, c
         misaligned(scratch, 16))
         return PSPMM_E_ARG;
     char *base = (char *)scratch;
-    uint32_t *keys[2], *pos[2];
-    for (int i = 0; i < 2; ++i) {
-        keys[i] = (uint32_t *)(base + lay.keys[i]);
-        pos[i] = (uint32_t *)(base + lay.pos[i]);
+    uint2 *pairs[2] = {(uint2 *)(base + lay.pairs[0]), (uint2 *)(base + lay.pairs[1])};
+    const int32_t tiles = (int32_t)((n + TILE - 1) / TILE);
+    uint32_t *counts = (uint32_t *)(base + lay.counts);
+    int bits = 1;
+    while (bits < 32 && (n_rows >> bits) != 0)
+        ++bits;  // keys are 0 .. n_rows
+    const int passes = n <= RANK_MAX ? 0 : (bits + 7) / 8, digit = passes ? (bits + passes - 1) / passes : 0;
+    // The counts before a tile: read by each up to this many tiles (tiles^2 KB in all), else scanned by a launch of its own.
+    const bool scan = tiles > SCAN_TILES;
+    SortArgs s = {{ids, n, n_rows, padding, ids64 != 0}, nullptr, pairs[0], counts, scan ? (uint32_t *)(base + lay.totals) : nullptr,
+                  nullptr, tiles, 0, passes, digit, (1 << digit) - 1, 0, {}};
+    s.fill = {(char *)out, n_rows * dim * B, 0, passes ? 1 + (scan ? 2 : 1) * passes : 1, 0};
+    if (ld_out != dim) {  // (rows apart from one another)
+        PSPMM_CUDA_TRY(cudaMemset2DAsync(out, (size_t)ld_out * B, 0, (size_t)dim * B, (size_t)n_rows, st));
+        s.fill.bytes = 0;
     }
-    SortArgs s = {{ids, n, n_rows, padding, ids64 != 0}, nullptr, nullptr, keys[0], pos[0], (uint32_t *)(base + lay.counts),
-                  (uint32_t *)(base + lay.totals), (int32_t)((n + TILE - 1) / TILE), 0};
+    // CTAs that fill: 16 KB each, or two per SM
+    const int64_t fill = (s.fill.bytes / s.fill.shares + (16 << 10) - 1) >> 14, most = 2 * (int64_t)pspmm_sm_count();
+    s.fill.ctas = (int32_t)(fill < 1 ? 1 : fill < most ? fill : most);
+    // (the first launch waits for all before it; the others, for one another where they need to)
+    auto first = [&](void (*kern)(const SortArgs), int work) {
+        s.work = work;
+        kern<<<(unsigned)(work + s.fill.ctas), 256, 0, st>>>(s);
+        ++s.fill.share;
+        return cudaGetLastError();
+    };
+    auto then = [&](void (*kern)(const SortArgs), int work) {
+        s.work = work;
+        const cudaError_t e = launch_dependent(kern, dim3((unsigned)(work + s.fill.ctas)), 256, 0, st, s);
+        ++s.fill.share;
+        return e;
+    };
+    PSPMM_CUDA_TRY(passes ? first(digit_count_kernel, tiles) : first(rank_kernel, (int)((n + 7) / 8)));
     int last = 0;
-    if (n <= RANK_MAX) {
-        rank_kernel<<<(unsigned)((n + 7) / 8), 256, 0, st>>>(s);
-        PSPMM_CUDA_TRY(cudaGetLastError());
-    } else {
-        int bits = 1;
-        while (bits < 32 && (n_rows >> bits) != 0)
-            ++bits;  // keys are 0 .. n_rows
-        for (int p = 0; p * 8 < bits; ++p) {
-            s.key_in = p ? keys[last] : nullptr;
-            s.pos_in = p ? pos[last] : nullptr;
-            last = p ? last ^ 1 : 0;
-            s.key_out = keys[last];
-            s.pos_out = pos[last];
-            s.shift = 8 * p;
-            digit_count_kernel<<<s.tiles, TILE_THREADS, 0, st>>>(s);
-            PSPMM_CUDA_TRY(cudaGetLastError());
-            digit_scan_kernel<<<256, 256, 0, st>>>(s);
-            PSPMM_CUDA_TRY(cudaGetLastError());
-            digit_scatter_kernel<<<s.tiles, TILE_THREADS, 0, st>>>(s);
-            PSPMM_CUDA_TRY(cudaGetLastError());
-        }
+    for (int p = 0; p < passes; ++p) {
+        s.from = p ? pairs[last] : nullptr;
+        last = p ? last ^ 1 : 0;
+        s.to = pairs[last];
+        s.shift = digit * p;
+        s.counts = counts + (int64_t)p * tiles * 256;
+        s.next = p + 1 < passes ? s.counts + (int64_t)tiles * 256 : nullptr;
+        if (scan)
+            PSPMM_CUDA_TRY(then(digit_scan_kernel, 256));
+        PSPMM_CUDA_TRY(then(digit_scatter_kernel, tiles));
     }
-    const GradArgs a = {keys[last], pos[last], grad, out, (float *)(base + lay.part), n, n_rows, ld_grad, ld_out, 0, 0,
-                        run_for(n), 0, 0, 0, 0, dim, scale};
+    const GradArgs a = {pairs[last], grad, out, (float *)(base + lay.part), n, n_rows, ld_grad, ld_out, 0, run_for(n), 0, 0, dim, 0, scale};
     PSPMM_CUDA_TRY(dtype == PSPMM_F32    ? grad_typed<float>(a, dim, st)
                    : dtype == PSPMM_BF16 ? grad_typed<bf16>(a, dim, st)
                                          : grad_typed<f16>(a, dim, st));
