@@ -42,7 +42,8 @@ struct Ids {
 struct Fill {
     char *p;
     int64_t bytes;
-    int32_t share, shares, ctas;
+    int32_t share, shares, ctas;  // shares done, and in all
+    int32_t now;                  // shares of this launch
 };
 
 // Sorted and unsorted ids are pairs: sort key in x, position in y.
@@ -157,7 +158,7 @@ __device__ __forceinline__ void fill_zeros(const Fill &f, int cta)
 {
     const int64_t lead = min((int64_t)(-(uintptr_t)f.p & 15), f.bytes), whole = (f.bytes - lead) / 16;
     uint4 *p = reinterpret_cast<uint4 *>(f.p + lead);
-    const int64_t from = whole * f.share / f.shares, to = whole * (f.share + 1) / f.shares;
+    const int64_t from = whole * f.share / f.shares, to = whole * (f.share + f.now) / f.shares;
     for (int64_t i = from + (int64_t)cta * 256 + threadIdx.x; i < to; i += (int64_t)f.ctas * 256)
         p[i] = make_uint4(0, 0, 0, 0);
     if (f.share == 0 && cta == 0) {  // the ends (elements of 2 or 4 bytes)
@@ -282,8 +283,8 @@ __global__ void __launch_bounds__(256) digit_scan_kernel(const SortArgs a)
         a.totals[blockIdx.x] = carry;
 }
 
-// Stable: a warp takes 256 neighbouring keys, 32 at a time; equal digits among the 32 find one another by a match, and a
-// count per warp and digit carries on from one 32 to the next.  The tile is put in order in shared memory, so that equal digits leave
+// Stable: a warp takes 256 neighbouring keys, 32 at a time; equal digits among the 32 find one another by a ballot per bit (a
+// third of what a match instruction takes), and a count per warp and digit carries on from one 32 to the next.  The tile is put in order in shared memory, so that equal digits leave
 // side by side.
 __global__ void __launch_bounds__(TILE_THREADS) digit_scatter_kernel(const SortArgs a)
 {
@@ -323,8 +324,12 @@ __global__ void __launch_bounds__(TILE_THREADS) digit_scatter_kernel(const SortA
 #pragma unroll
     for (int k = 0; k < TILE_KEYS; ++k) {
         const bool in = i0 + k * 32 < a.in.n;
-        const uint32_t d = in ? pair[k].x >> a.shift & a.mask : 256;  // (lanes beyond the end match one another only)
-        const uint32_t same = __match_any_sync(PSPMM_FULL_MASK, d);
+        const uint32_t d = in ? pair[k].x >> a.shift & a.mask : 0;
+        uint32_t same = __ballot_sync(PSPMM_FULL_MASK, in);
+        for (int b = 0; b < a.bits; ++b) {
+            const uint32_t set = __ballot_sync(PSPMM_FULL_MASK, d >> b & 1);
+            same &= d >> b & 1 ? set : ~set;
+        }
         const uint32_t below = __popc(same & ((1u << lane) - 1));
         rank[k] = in ? seen[warp][d] + below : 0;
         __syncwarp();
@@ -359,30 +364,21 @@ __global__ void __launch_bounds__(TILE_THREADS) digit_scatter_kernel(const SortA
             a.to[to] = v;
             place = (uint32_t)count_at(a, to / TILE, v.x >> (a.shift + a.bits) & a.mask);
         }
-        if (a.next) {  // (hot ids and short last digits would have the lanes add to one place in turn)
-            const uint32_t same = __match_any_sync(PSPMM_FULL_MASK, place);
-            if (place != 0xffffffffu && (same & ((1u << lane) - 1)) == 0)
-                atomicAdd(&a.next[place], (uint32_t)__popc(same));
+        if (a.next) {
+            // A hot id's keys lie side by side: one addition for neighbours with one place (in turn, additions to a place take 50 ns each).
+            const uint32_t left = __shfl_up_sync(PSPMM_FULL_MASK, place, 1);
+            const uint32_t heads = __ballot_sync(PSPMM_FULL_MASK, lane == 0 || place != left);
+            if (place != 0xffffffffu && (heads >> lane & 1)) {
+                const uint32_t behind = lane == 31 ? 0 : heads >> (lane + 1);
+                atomicAdd(&a.next[place], behind ? (uint32_t)__ffs(behind) : (uint32_t)(32 - lane));
+            }
         }
     }
 }
 
 // ---- sums ----------------------------------------------------------------------------------------------------------
 
-// First position in [lo, hi) whose key is not below `key` (hi: none).
-__device__ __forceinline__ int64_t lower_bound(const uint2 *ids, uint32_t key, int64_t lo, int64_t hi)
-{
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (ids[mid].x < key)
-            lo = mid + 1;
-        else
-            hi = mid;
-    }
-    return lo;
-}
-
-// The same over [lo, n) by a whole warp, 32 probes a step.
+// First position in [lo, n) whose key is not below `key` (n: none), by a whole warp, 32 probes a step.
 __device__ __forceinline__ int64_t warp_lower_bound(const uint2 *ids, uint32_t key, int64_t lo, int64_t n)
 {
     const int lane = threadIdx.x % 32;
@@ -490,7 +486,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const GradArgs a)
         const uint32_t key = ids[next].x;
         if (key >= a.n_rows || ids[next - 1].x != key)
             return;
-        const int64_t s = lower_bound(ids, key, first, next);
+        const int64_t s = warp_lower_bound(ids, key, first, next);
         if (s == first && first > 0 && ids[first - 1].x == key)
             return;
         const int64_t c0 = s / a.run;
@@ -528,13 +524,13 @@ __global__ void __launch_bounds__(256) combine_kernel(const GradArgs a)
     const uint32_t key = ids[end].x;
     if (key >= a.n_rows || ids[end - 1].x != key)
         return;
-    const int64_t s = lower_bound(ids, key, begin, end);
+    const int64_t s = warp_lower_bound(ids, key, begin, end);
     if (s == begin && begin > 0 && ids[begin - 1].x == key)
         return;
     const int64_t far = (chunk + HOT) * a.run;
     if (far < a.n && ids[far].x == key)
         return;
-    const int64_t c1 = (lower_bound(ids, key + 1, end, far < a.n ? far : a.n) - 1) / a.run;
+    const int64_t c1 = (warp_lower_bound(ids, key + 1, end, far < a.n ? far : a.n) - 1) / a.run;
     const int col = (int)(unit % tiles) * 128 + lane;
     float sum[4] = {};
     for (int64_t c0 = chunk; c0 <= c1; c0 += 4) {
@@ -563,11 +559,12 @@ __global__ void __launch_bounds__(256) combine_kernel(const GradArgs a)
 
 template <typename T, int VW, int L> cudaError_t launch_lookup_lanes(const LookupArgs &a, cudaStream_t st)
 {
-    constexpr int MOST = L < 8 ? L : 8;
-    const int64_t groups = 256 / L, ctas = (a.n + groups - 1) / groups;
+    const int64_t groups = 256 / L, ctas = (a.n + groups - 1) / groups, enough = 4 * (int64_t)pspmm_sm_count();
     // several rows per lane group where that still leaves every SM some CTAs
-    if (ctas >= MOST * 4 * (int64_t)pspmm_sm_count())
-        lookup_kernel<T, VW, L, MOST><<<(unsigned)((ctas + MOST - 1) / MOST), 256, 0, st>>>(a);
+    if (L >= 8 && ctas >= 8 * enough)
+        lookup_kernel<T, VW, L, L < 8 ? L : 8><<<(unsigned)((ctas + 7) / 8), 256, 0, st>>>(a);
+    else if (ctas >= 4 * enough)
+        lookup_kernel<T, VW, L, 4><<<(unsigned)((ctas + 3) / 4), 256, 0, st>>>(a);
     else
         lookup_kernel<T, VW, L, 1><<<(unsigned)ctas, 256, 0, st>>>(a);
     return cudaGetLastError();
@@ -728,13 +725,13 @@ extern "C" int pspmm_embedding_grad(const void *ids, int32_t ids64, int64_t n, c
     const bool scan = tiles > SCAN_TILES;
     SortArgs s = {{ids, n, n_rows, padding, ids64 != 0}, nullptr, pairs[0], counts, scan ? (uint32_t *)(base + lay.totals) : nullptr,
                   nullptr, tiles, 0, passes, digit, (1 << digit) - 1, 0, {}};
-    s.fill = {(char *)out, n_rows * dim * B, 0, passes ? 1 + (scan ? 2 : 1) * passes : 1, 0};
+    s.fill = {(char *)out, n_rows * dim * B, 0, passes ? 1 + (scan ? 3 : 2) * passes : 1, 0, 1};
     if (ld_out != dim) {  // (rows apart from one another)
         PSPMM_CUDA_TRY(cudaMemset2DAsync(out, (size_t)ld_out * B, 0, (size_t)dim * B, (size_t)n_rows, st));
         s.fill.bytes = 0;
     }
-    // CTAs that fill: 16 KB each, or two per SM
-    const int64_t fill = (s.fill.bytes / s.fill.shares + (16 << 10) - 1) >> 14, most = 2 * (int64_t)pspmm_sm_count();
+    // CTAs that fill: 16 KB each, or four per SM.  The passes' placing takes longest and has two shares.
+    const int64_t fill = (s.fill.bytes / s.fill.shares + (16 << 10) - 1) >> 14, most = 4 * (int64_t)pspmm_sm_count();
     s.fill.ctas = (int32_t)(fill < 1 ? 1 : fill < most ? fill : most);
     // (the first launch waits for all before it; the others, for one another where they need to)
     auto first = [&](void (*kern)(const SortArgs), int work) {
@@ -743,10 +740,11 @@ extern "C" int pspmm_embedding_grad(const void *ids, int32_t ids64, int64_t n, c
         ++s.fill.share;
         return cudaGetLastError();
     };
-    auto then = [&](void (*kern)(const SortArgs), int work) {
+    auto then = [&](void (*kern)(const SortArgs), int work, int shares) {
         s.work = work;
+        s.fill.now = shares;
         const cudaError_t e = launch_dependent(kern, dim3((unsigned)(work + s.fill.ctas)), 256, 0, st, s);
-        ++s.fill.share;
+        s.fill.share += shares;
         return e;
     };
     PSPMM_CUDA_TRY(passes ? first(digit_count_kernel, tiles) : first(rank_kernel, (int)((n + 7) / 8)));
@@ -759,8 +757,8 @@ extern "C" int pspmm_embedding_grad(const void *ids, int32_t ids64, int64_t n, c
         s.counts = counts + (int64_t)p * tiles * 256;
         s.next = p + 1 < passes ? s.counts + (int64_t)tiles * 256 : nullptr;
         if (scan)
-            PSPMM_CUDA_TRY(then(digit_scan_kernel, 256));
-        PSPMM_CUDA_TRY(then(digit_scatter_kernel, tiles));
+            PSPMM_CUDA_TRY(then(digit_scan_kernel, 256, 1));
+        PSPMM_CUDA_TRY(then(digit_scatter_kernel, tiles, 2));
     }
     const GradArgs a = {pairs[last], grad, out, (float *)(base + lay.part), n, n_rows, ld_grad, ld_out, 0, run_for(n), 0, 0, dim, 0, scale};
     PSPMM_CUDA_TRY(dtype == PSPMM_F32    ? grad_typed<float>(a, dim, st)

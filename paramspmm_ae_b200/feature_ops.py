@@ -20,10 +20,10 @@ EIGHT_BLOCK = 128  # columns that share a scale in the 8-bit form
 MAX_DIM = 1 << 24
 
 
-def _gpu_of(*tensors):
-    """The one device of the operands (None among them: left out)."""
+def _check_tensors(**tensors):
+    """What is wrong with operands that are not tensors of one GPU (None among them: left out)."""
     gpu = None
-    for name, t in tensors:
+    for name, t in tensors.items():
         if t is None:
             continue
         if not isinstance(t, torch.Tensor):
@@ -34,7 +34,11 @@ def _gpu_of(*tensors):
             gpu = t.get_device()
         elif t.get_device() != gpu:
             raise RuntimeError("%s is on another device than the other operands" % name)
-    return gpu
+
+
+def _gpu(t):
+    """The GPU of a tensor; -1 for anything else."""
+    return t.get_device() if isinstance(t, torch.Tensor) and t.is_cuda else -1
 
 
 def _elsewhere(gpu):
@@ -46,15 +50,16 @@ def _rows(t, name, dtype=None, shape=None):
     dimensions taken as rows of its last one."""
     if t.dtype not in _DTYPES or (dtype is not None and t.dtype is not dtype):
         raise RuntimeError("%s must have dtype %s, got %s" % (name, dtype or "float32, bfloat16 or float16", t.dtype))
-    if shape is not None and t.shape != shape:
-        raise RuntimeError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
-    if t.dim() == 0 or t.shape[-1] == 0 or t.shape[-1] > MAX_DIM:
+    size = t.shape
+    if shape is not None and size != shape:
+        raise RuntimeError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(size)))
+    dim = size[-1] if size else 0
+    if not 0 < dim <= MAX_DIM:
         raise RuntimeError("%s must have between 1 and %d columns" % (name, MAX_DIM))
-    dim = t.shape[-1]
     if t.is_contiguous():
         return t.numel() // dim, dim, dim
     if t.dim() == 2 and (t.stride(1) == 1 or dim == 1) and t.stride(0) >= dim:
-        return t.shape[0], dim, t.stride(0)
+        return size[0], dim, t.stride(0)
     raise RuntimeError("%s must be contiguous, or a matrix whose rows are" % name)
 
 
@@ -76,7 +81,9 @@ def embedding(ids, table, scale=1.0):
     """``scale * table[ids]``: one row of ``table`` ([rows, dim]) per id, of the table's type, shaped ``ids.shape + (dim,)``.
 
     An id outside the table gives a row of NaN and sets :func:`embedding_status` (the GPU is not waited for)."""
-    gpu = _gpu_of(("ids", ids), ("table", table))
+    gpu = _gpu(table)
+    if gpu < 0 or _gpu(ids) != gpu:
+        _check_tensors(ids=ids, table=table)
     if _elsewhere(gpu):
         with torch.cuda.device(gpu):
             return embedding(ids, table, scale)
@@ -84,7 +91,7 @@ def embedding(ids, table, scale=1.0):
     if table.dim() != 2:
         raise RuntimeError("table must be 2-dimensional")
     rows, dim, ld = _rows(table, "table")
-    out = torch.empty(ids.shape + (dim,), dtype=table.dtype, device=table.device)
+    out = table.new_empty(ids.shape + (dim,))
     rc = lib().pspmm_embedding(ids.data_ptr(), wide, ids.numel(), table.data_ptr(), _DTYPES[table.dtype], rows, dim, ld, scale,
                                out.data_ptr(), dim, _stream())
     if rc:
@@ -97,7 +104,9 @@ def embedding_grad(ids, grad, n_rows, scale=1.0, padding_idx=None):
     ``grad`` whose id is t, of the type of ``grad``; ids equal to ``padding_idx`` and ids outside the table add nothing.
 
     The sums run in the order of the ids' positions (they are sorted first): equal calls give equal bits."""
-    gpu = _gpu_of(("ids", ids), ("grad", grad))
+    gpu = _gpu(grad)
+    if gpu < 0 or _gpu(ids) != gpu:
+        _check_tensors(ids=ids, grad=grad)
     if _elsewhere(gpu):
         with torch.cuda.device(gpu):
             return embedding_grad(ids, grad, n_rows, scale, padding_idx)
@@ -109,7 +118,7 @@ def embedding_grad(ids, grad, n_rows, scale=1.0, padding_idx=None):
         raise RuntimeError("n_rows must not be negative")
     if padding_idx is not None and not 0 <= padding_idx < n_rows:
         raise RuntimeError("padding_idx must be a row of the table")
-    out = torch.empty((n_rows, dim), dtype=grad.dtype, device=grad.device)
+    out = grad.new_empty((n_rows, dim))
     scratch, need = _scratch("pspmm_embedding_grad_scratch_bytes", (n, dim), grad.device)
     rc = lib().pspmm_embedding_grad(ids.data_ptr(), wide, n, grad.data_ptr(), _DTYPES[grad.dtype], ld, n_rows, dim, scale,
                                     -1 if padding_idx is None else padding_idx, out.data_ptr(), dim, _ptr(scratch), need, _stream())
@@ -154,13 +163,15 @@ class Rows8:
 
     def dequantize(self, dtype=torch.float32):
         """The values that the whole numbers stand for."""
-        gpu = _gpu_of(("q", self.q), ("scales", self.scales))
+        gpu = _gpu(self.q)
+        if gpu < 0:
+            _check_tensors(q=self.q)
         if _elsewhere(gpu):
             with torch.cuda.device(gpu):
                 return self.dequantize(dtype)
         if dtype not in _DTYPES:
             raise RuntimeError("dtype must be float32, bfloat16 or float16, got %s" % dtype)
-        out = torch.empty(self.shape, dtype=dtype, device=self.q.device)
+        out = self.q.new_empty(self.shape, dtype=dtype)
         rc = lib().pspmm_dequantize_rows(self.q.data_ptr(), self.q.shape[1], self.scales.data_ptr(), _DTYPES[dtype], out.data_ptr(),
                                          self.dim, self.q.shape[0], self.dim, _stream())
         if rc:
@@ -172,23 +183,30 @@ class Rows8:
         return rows8_mm_t(self, G)
 
 
-def _empty_rows8(n, dim, device):
-    return (torch.empty((n, dim + -dim % 16), dtype=torch.int8, device=device),
-            torch.empty((n, (dim + EIGHT_BLOCK - 1) // EIGHT_BLOCK), dtype=torch.float32, device=device))
+def _empty_rows8(x, n, dim):
+    """Rows8 of an array like ``x``, yet to be written."""
+    kept = Rows8.__new__(Rows8)
+    kept.q = x.new_empty((n, dim + -dim % 16), dtype=torch.int8)
+    kept.scales = x.new_empty((n, (dim + EIGHT_BLOCK - 1) // EIGHT_BLOCK), dtype=torch.float32)
+    kept.dim, kept.shape = dim, x.shape
+    return kept
 
 
 def quantize_rows(x):
     """``x`` in 8 bits (:class:`Rows8`), a scale per row and 128 columns."""
-    gpu = _gpu_of(("x", x))
+    gpu = _gpu(x)
+    if gpu < 0:
+        _check_tensors(x=x)
     if _elsewhere(gpu):
         with torch.cuda.device(gpu):
             return quantize_rows(x)
     n, dim, ld = _rows(x, "x")
-    q, scales = _empty_rows8(n, dim, x.device)
-    rc = lib().pspmm_quantize_rows(x.data_ptr(), _DTYPES[x.dtype], ld, n, dim, q.data_ptr(), q.shape[1], scales.data_ptr(), _stream())
+    kept = _empty_rows8(x, n, dim)
+    rc = lib().pspmm_quantize_rows(x.data_ptr(), _DTYPES[x.dtype], ld, n, dim, kept.q.data_ptr(), dim + -dim % 16,
+                                   kept.scales.data_ptr(), _stream())
     if rc:
         check(rc)
-    return Rows8(q, scales, dim, x.shape)
+    return kept
 
 
 def rows8_mm_t(rows, G, out=None):
@@ -196,7 +214,9 @@ def rows8_mm_t(rows, G, out=None):
     gradient of a layer that kept its input in 8 bits, on the tensor cores with float32 accuracy."""
     if not isinstance(rows, Rows8):
         raise RuntimeError("rows must be a Rows8")
-    gpu = _gpu_of(("q", rows.q), ("scales", rows.scales), ("G", G), ("out", out))
+    gpu = _gpu(G)
+    if gpu < 0 or _gpu(rows.q) != gpu or (out is not None and _gpu(out) != gpu):
+        _check_tensors(q=rows.q, G=G, out=out)
     if _elsewhere(gpu):
         with torch.cuda.device(gpu):
             return rows8_mm_t(rows, G, out)
@@ -204,7 +224,7 @@ def rows8_mm_t(rows, G, out=None):
     if n != rows.q.shape[0]:
         raise RuntimeError("G must have one row per row held, %d, got %d" % (rows.q.shape[0], n))
     if out is None:
-        out = torch.empty((rows.dim, cols), dtype=torch.float32, device=G.device)
+        out = G.new_empty((rows.dim, cols), dtype=torch.float32)
     elif (out.dtype is not torch.float32 or out.shape != (rows.dim, cols) or out.stride(1) != 1 or out.stride(0) < cols):
         raise RuntimeError("out must be a float32 matrix of %d rows of %d with unit column stride" % (rows.dim, cols))
     aligned = 1 if (ld * G.element_size()) % 16 == 0 and G.data_ptr() % 16 == 0 else 0
@@ -238,7 +258,9 @@ def rms_norm(x, weight, residual=None, eps=1e-6, relu=False, values=True, eight_
     Returns ``(y, h, rstd, kept)``: ``h`` is the residual stream (``x`` itself without a ``residual``), ``rstd`` (float32, one per
     row) what :func:`rms_norm_backward` needs, ``kept`` the :class:`Rows8` of ``y`` with ``eight_bit`` (else None), made in the
     same pass.  ``values=False`` leaves ``y`` out (None) for a consumer of the 8 bits alone."""
-    gpu = _gpu_of(("x", x), ("weight", weight), ("residual", residual))
+    gpu = _gpu(x)
+    if gpu < 0 or _gpu(weight) != gpu or (residual is not None and _gpu(residual) != gpu):
+        _check_tensors(x=x, weight=weight, residual=residual)
     if _elsewhere(gpu):
         with torch.cuda.device(gpu):
             return rms_norm(x, weight, residual, eps, relu, values, eight_bit)
@@ -248,27 +270,31 @@ def rms_norm(x, weight, residual=None, eps=1e-6, relu=False, values=True, eight_
         raise RuntimeError("eps must not be negative")
     if not values and not eight_bit:
         raise RuntimeError("nothing is asked for: neither values nor the 8-bit form")
-    h, ld_r = x, 0
+    h, ld_r, r_ptr, h_ptr = x, 0, None, None
     if residual is not None:
         ld_r = _rows(residual, "residual", x.dtype, x.shape)[2]
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if values else None
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    q = scales = None
+        h = x.new_empty(x.shape)
+        r_ptr, h_ptr = residual.data_ptr(), h.data_ptr()
+    y = x.new_empty(x.shape) if values else None
+    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    kept, q_ptr, s_ptr = None, None, None
     if eight_bit:
-        q, scales = _empty_rows8(n, dim, x.device)
-    rc = lib().pspmm_rms_norm(x.data_ptr(), ld, _ptr(residual), ld_r, weight.data_ptr(), _DTYPES[x.dtype], n, dim, eps,
-                              1 if relu else 0, None if residual is None else h.data_ptr(), dim, _ptr(y), dim, rstd.data_ptr(),
-                              _ptr(q), q.shape[1] if eight_bit else 0, _ptr(scales), _stream())
+        kept = _empty_rows8(x, n, dim)
+        q_ptr, s_ptr = kept.q.data_ptr(), kept.scales.data_ptr()
+    rc = lib().pspmm_rms_norm(x.data_ptr(), ld, r_ptr, ld_r, weight.data_ptr(), _DTYPES[x.dtype], n, dim, eps, 1 if relu else 0,
+                              h_ptr, dim, y.data_ptr() if values else None, dim, rstd.data_ptr(), q_ptr, dim + -dim % 16, s_ptr,
+                              _stream())
     if rc:
         check(rc)
-    return y, h, rstd, Rows8(q, scales, dim, x.shape) if eight_bit else None
+    return y, h, rstd, kept
 
 
 def rms_norm_backward(dy, h, rstd, weight, dh=None, relu=False):
     """Gradients ``(dx, dweight)`` of :func:`rms_norm` from ``dy`` and, where the residual stream goes on, the gradient ``dh`` that
     reaches ``h`` itself; ``dx`` is the gradient of ``x`` and of ``residual`` alike."""
-    gpu = _gpu_of(("dy", dy), ("h", h), ("rstd", rstd), ("weight", weight), ("dh", dh))
+    gpu = _gpu(dy)
+    if gpu < 0 or _gpu(h) != gpu or _gpu(rstd) != gpu or _gpu(weight) != gpu or (dh is not None and _gpu(dh) != gpu):
+        _check_tensors(dy=dy, h=h, rstd=rstd, weight=weight, dh=dh)
     if _elsewhere(gpu):
         with torch.cuda.device(gpu):
             return rms_norm_backward(dy, h, rstd, weight, dh, relu)
@@ -278,8 +304,8 @@ def rms_norm_backward(dy, h, rstd, weight, dh=None, relu=False):
     _vector(weight, "weight", dim, h.dtype)
     if rstd.dtype is not torch.float32 or rstd.shape != h.shape[:-1] or not rstd.is_contiguous():
         raise RuntimeError("rstd must be contiguous float32, one per row")
-    dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-    dw = torch.empty_like(weight)
+    dx = h.new_empty(h.shape)
+    dw = weight.new_empty(dim)
     scratch, need = _scratch("pspmm_rms_norm_backward_scratch_bytes", (n, dim), h.device)
     rc = lib().pspmm_rms_norm_backward(dy.data_ptr(), ld_dy, h.data_ptr(), ld_h, rstd.data_ptr(), weight.data_ptr(), _ptr(dh), ld_dh,
                                        _DTYPES[h.dtype], n, dim, 1 if relu else 0, dx.data_ptr(), dim, dw.data_ptr(), _ptr(scratch),
