@@ -63,6 +63,14 @@ __device__ __forceinline__ uint32_t eight_round(double x, double up)
 {
     return (uint32_t)__double2loint(fma(x, up, 6755399441055744.0));
 }
+// The same for x + low, low what x's rounding left of it.
+__device__ __forceinline__ uint32_t eight_round(float x, float low, float up)
+{
+    const float z = x * up, ez = fmaf(low, up, fmaf(x, up, -z));
+    const float m = z + 12582912.f;
+    const float d = z - (m - 12582912.f);  // from the whole number that z is nearest to; exact, as 1/2 - d is where it matters
+    return __float_as_uint(m) + (ez > 0.5f - d ? 1u : 0u) - (ez < -0.5f - d ? 1u : 0u);
+}
 __device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);

@@ -5,12 +5,16 @@
 //
 // Bound by HBM: every array is moved once.  A row is held in the registers of its lanes between the sum and its use: 8, 16 or
 // 32 lanes (several rows per warp) with up to 16 values each, a CTA of 64 to 1,024 threads beyond that, and two passes over a row
-// wider than 8,192 columns.
+// wider than 8,192 columns.  Rows of a CTA wait at a barrier between their sum and its use, so each asks for the row after the next
+// to be brought to L2.  x + r -> h, y in us (TB/s), alone, with y in 8 bits beside, and backward: 169,343 x 128 fp32
+// 66 (5.3), 72, 64; 16,384 x 4,096 bf16 120 (4.5), 217, 104; single values, 30,000 x 2,047 fp32 221 (4.4), 538, 193.  The 8-bit forms of
+// wide rows are bound by the instructions of the second number.  Rows brought to shared memory by bulk copies, several
+// in flight per CTA, were slower but for those (bf16 127, 210, 159): one more pass of instructions over every value.
 //
-// Numbers: the squares are added in 64 bits, which costs nothing here (the 64-bit units run at half the 32-bit rate and the memory
-// system leaves them idle).  y in 8 bits is taken from h, rstd and y in 64 bits throughout, because next to a half the last bit of
-// a 32-bit y decides which whole number it becomes; y itself is the 32-bit one with and without it.  rstd is kept in 32 bits for the
-// backward, whose sums are in 32 bits.
+// Numbers: h = x + r is squared and added in 64 bits; rstd is kept in 32 bits for the backward, whose sums are in 32 bits.  y in 8 bits is
+// taken from a y with twice the bits of a 32-bit one, because next to a half the last bit of that decides which whole number it becomes;
+// y itself is the 32-bit one with and without it.  Those bits are a second 32-bit number (values below 1e-30 have fewer): in 64-bit
+// numbers the norm of 169,343 x 128 took 92 us against 66, most of it conversions, of which an SM does 16 per clock.
 #include "feature_types.cuh"
 
 namespace {
@@ -41,6 +45,8 @@ struct WeightArgs {
     void *dw;
     int32_t parts, dim, dtype;
 };
+
+constexpr int AHEAD = 2;  // rows of a lane group that are brought to L2
 
 // TPR threads share a row; each holds VPT vectors of VW values.
 template <int TPR> struct Rows {
@@ -98,6 +104,27 @@ __device__ __forceinline__ uint32_t group_mask(int lanes)
     return lanes == 32 ? PSPMM_FULL_MASK : ((1u << lanes) - 1) << (threadIdx.x % 32 / lanes * lanes);
 }
 
+// 1 / sqrt(m) in 64 bits: the 32-bit one and two steps of Newton's, which double its correct bits (the library's quotient of a root
+// took a third of the narrow rows' time).  Outside the 32-bit numbers' range, the library's.
+__device__ __forceinline__ double inverse_root(double m)
+{
+    if (!(m > 1e-30 && m < 1e30))
+        return 1.0 / sqrt(m);
+    double r = (double)rsqrtf((float)m);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        r = fma(r * 0.5, fma(-m * r, r, 1.0), r);
+    return r;
+}
+
+// A row to come is brought to L2, so that its loads wait for that and not for memory.
+__device__ __forceinline__ void look_ahead(const void *row, int bytes)
+{
+    const uintptr_t from = ((uintptr_t)row + 15) / 16 * 16, to = ((uintptr_t)row + bytes) / 16 * 16;
+    if (from < to)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"((uint32_t)(to - from)) : "memory");
+}
+
 template <typename T, int VW, int TPR, int VPT, bool EIGHT>
 __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs a)
 {
@@ -111,31 +138,43 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs
         const int c = column<VW, TPR, VPT>(t, v);
         load_some<T, VW>(w[v], static_cast<const T *>(a.w) + c, c < a.dim);
     }
-    for (int64_t row = (int64_t)blockIdx.x * R::PER_CTA + threadIdx.x / TPR; row < a.n; row += (int64_t)gridDim.x * R::PER_CTA) {
-        float x[VPT][VW], r[VPT][VW];
+    const int64_t step = (int64_t)gridDim.x * R::PER_CTA;
+    for (int64_t row = (int64_t)blockIdx.x * R::PER_CTA + threadIdx.x / TPR; row < a.n; row += step) {
+        float h[VPT][VW], low[VPT][VW];  // x + r in 32 bits, and what that leaves of the residual until it is added
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
             const int c = column<VW, TPR, VPT>(t, v);
-            load_some<T, VW>(x[v], static_cast<const T *>(a.x) + row * a.ld_x + c, c < a.dim);
+            load_some<T, VW>(h[v], static_cast<const T *>(a.x) + row * a.ld_x + c, c < a.dim);
         }
         if (a.r) {
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
                 const int c = column<VW, TPR, VPT>(t, v);
-                load_some<T, VW>(r[v], static_cast<const T *>(a.r) + row * a.ld_r + c, c < a.dim);
+                load_some<T, VW>(low[v], static_cast<const T *>(a.r) + row * a.ld_r + c, c < a.dim);
             }
         }
-        double ss = 0, ss64 = 0;
-        float h[VPT][VW];
+        if (TPR > 32 && t == 0 && row + AHEAD * step < a.n) {
+            look_ahead(static_cast<const T *>(a.x) + (row + AHEAD * step) * a.ld_x, a.dim * (int)sizeof(T));
+            if (a.r)
+                look_ahead(static_cast<const T *>(a.r) + (row + AHEAD * step) * a.ld_r, a.dim * (int)sizeof(T));
+        }
+        double ss = 0;
 #pragma unroll
         for (int v = 0; v < VPT; ++v)
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
-                h[v][i] = a.r ? x[v][i] + r[v][i] : x[v][i];
-                ss = fma((double)h[v][i], (double)h[v][i], ss);
-                if constexpr (EIGHT) {
-                    const double h64 = a.r ? (double)x[v][i] + (double)r[v][i] : (double)x[v][i];
-                    ss64 = fma(h64, h64, ss64);
+                if (a.r) {
+                    const double h64 = (double)h[v][i] + (double)low[v][i];
+                    ss = fma(h64, h64, ss);
+                    const float x = h[v][i], r = low[v][i];
+                    h[v][i] = x + r;
+                    if constexpr (EIGHT) {  // the exact remainder of a sum (Knuth's)
+                        const float b = h[v][i] - x;
+                        low[v][i] = (x - (h[v][i] - b)) + (r - b);
+                    }
+                } else {
+                    ss = fma((double)h[v][i], (double)h[v][i], ss);
+                    low[v][i] = 0.f;
                 }
             }
         if (a.h) {
@@ -147,46 +186,54 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs
             }
         }
         ss = row_sum<double, TPR>(ss, mask, sums);
-        const float rstd = (float)(1.0 / sqrt(ss / a.dim + a.eps));
+        const double rstd64 = inverse_root(ss / a.dim + a.eps);
+        const float rstd = (float)rstd64;
         if (t == 0)
             a.rstd[row] = rstd;
         if (a.y) {
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
                 const int c = column<VW, TPR, VPT>(t, v);
+                float y[VW];
 #pragma unroll
                 for (int i = 0; i < VW; ++i) {
-                    h[v][i] = h[v][i] * rstd * w[v][i];  // y
-                    if (a.relu && h[v][i] < 0.f)
-                        h[v][i] = 0.f;
+                    y[i] = h[v][i] * rstd * w[v][i];
+                    if (a.relu && y[i] < 0.f)
+                        y[i] = 0.f;
                 }
                 if (c < a.dim)
-                    store_vec<T, VW>(static_cast<T *>(a.y) + row * a.ld_y + c, h[v]);
+                    store_vec<T, VW>(static_cast<T *>(a.y) + row * a.ld_y + c, y);
             }
         }
         if constexpr (EIGHT) {
+            // (h + low) rstd w as a sum of two 32-bit numbers, the first the sum rounded: products and what their rounding leaves (fma).
+            const float rest = (float)(rstd64 - rstd);
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int i = 0; i < VW; ++i) {
+                    const float n = h[v][i] * rstd;
+                    const float en = fmaf(low[v][i], rstd, fmaf(h[v][i], rest, fmaf(h[v][i], rstd, -n)));
+                    const float y = n * w[v][i];
+                    const float ey = fmaf(en, w[v][i], fmaf(n, w[v][i], -y));
+                    h[v][i] = y + ey;
+                    low[v][i] = (y - h[v][i]) + ey;
+                    if (a.relu && h[v][i] < 0.f)
+                        h[v][i] = low[v][i] = 0.f;
+                }
             // A block is LB lanes wide and SB vectors deep.
             constexpr int LB = R::LANES * VW >= EIGHT_BLOCK ? EIGHT_BLOCK / VW : R::LANES;
             constexpr int DEEP = EIGHT_BLOCK / (LB * VW), SB = DEEP < VPT ? DEEP : VPT;
             static_assert(VPT % SB == 0, "a block spans warps");
-            ss64 = row_sum<double, TPR>(ss64, mask, sums);
-            const double rstd64 = 1.0 / sqrt(ss64 / a.dim + a.eps);
             int8_t *q = a.q + row * a.pitch;
 #pragma unroll
             for (int v0 = 0; v0 < VPT; v0 += SB) {
-                double y[SB][VW];
                 uint32_t top = 0;
 #pragma unroll
-                for (int v = 0; v < SB; ++v)
+                for (int v = v0; v < v0 + SB; ++v)
 #pragma unroll
-                    for (int i = 0; i < VW; ++i) {
-                        const float xi = x[v0 + v][i];
-                        const double h64 = a.r ? (double)xi + (double)r[v0 + v][i] : (double)xi;
-                        y[v][i] = h64 * rstd64 * (double)w[v0 + v][i];
-                        if (a.relu && y[v][i] < 0.0)
-                            y[v][i] = 0.0;
-                        top = max(top, __float_as_uint((float)y[v][i]) & 0x7fffffffu);
-                    }
+                    for (int i = 0; i < VW; ++i)
+                        top = max(top, __float_as_uint(h[v][i]) & 0x7fffffffu);
 #pragma unroll
                 for (int d = LB / 2; d > 0; d >>= 1)
                     top = max(top, __shfl_xor_sync(mask, top, d));
@@ -196,12 +243,12 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs
                 if (first % EIGHT_BLOCK == 0 && first < a.dim)
                     a.scales[row * a.blocks + first / EIGHT_BLOCK] = scale;
 #pragma unroll
-                for (int v = 0; v < SB; ++v) {
-                    const int c = column<VW, TPR, VPT>(t, v0 + v);
+                for (int v = v0; v < v0 + SB; ++v) {
+                    const int c = column<VW, TPR, VPT>(t, v);
                     uint32_t b[VW];
 #pragma unroll
                     for (int i = 0; i < VW; ++i)
-                        b[i] = eight_round(y[v][i], (double)up);
+                        b[i] = eight_round(h[v][i], low[v][i], up);
                     if (c < a.pitch) {  // columns between dim and the pitch hold zeros
                         if constexpr (VW == 8)
                             *reinterpret_cast<uint2 *>(q + c) =
@@ -217,7 +264,7 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs
     }
 }
 
-// Rows of any width: a CTA per row, two passes.
+// Rows of any width: a CTA per row, two passes, 64-bit numbers.
 template <typename T, bool EIGHT>
 __global__ void __launch_bounds__(1024) norm_wide_kernel(const NormArgs a)
 {
@@ -226,21 +273,16 @@ __global__ void __launch_bounds__(1024) norm_wide_kernel(const NormArgs a)
     for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
         const T *x = static_cast<const T *>(a.x) + row * a.ld_x;
         const T *r = a.r ? static_cast<const T *>(a.r) + row * a.ld_r : nullptr;
-        double ss = 0, ss64 = 0;
+        double ss = 0;
         for (int c = threadIdx.x; c < a.dim; c += 1024) {
-            const float xi = to_float(x[c]), ri = r ? to_float(r[c]) : 0.f;
-            const float h = r ? xi + ri : xi;
-            const double h64 = r ? (double)xi + (double)ri : (double)xi;
-            ss = fma((double)h, (double)h, ss);
-            ss64 = fma(h64, h64, ss64);
+            const double h = r ? (double)to_float(x[c]) + (double)to_float(r[c]) : (double)to_float(x[c]);
+            ss = fma(h, h, ss);
         }
         ss = row_sum<double, 1024>(ss, PSPMM_FULL_MASK, sums);
-        const float rstd = (float)(1.0 / sqrt(ss / a.dim + a.eps));
+        const double rstd64 = inverse_root(ss / a.dim + a.eps);
+        const float rstd = (float)rstd64;
         if (threadIdx.x == 0)
             a.rstd[row] = rstd;
-        double rstd64 = 0;
-        if constexpr (EIGHT)
-            rstd64 = 1.0 / sqrt(row_sum<double, 1024>(ss64, PSPMM_FULL_MASK, sums) / a.dim + a.eps);
         // A warp takes 128 neighbouring columns at a time, a lane four of them.
         for (int c0 = threadIdx.x * 4; c0 < (a.dim + EIGHT_BLOCK - 1) / EIGHT_BLOCK * EIGHT_BLOCK; c0 += 4096) {
             double y64[4];
@@ -297,7 +339,14 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_backward_kernel(const
         const int c = column<VW, TPR, VPT>(t, v);
         load_some<T, VW>(w[v], static_cast<const T *>(a.w) + c, c < a.dim);
     }
-    for (int64_t row = (int64_t)blockIdx.x * R::PER_CTA + threadIdx.x / TPR; row < a.n; row += (int64_t)gridDim.x * R::PER_CTA) {
+    const int64_t step = (int64_t)gridDim.x * R::PER_CTA;
+    for (int64_t row = (int64_t)blockIdx.x * R::PER_CTA + threadIdx.x / TPR; row < a.n; row += step) {
+        if (TPR > 32 && t == 0 && row + AHEAD * step < a.n) {
+            look_ahead(static_cast<const T *>(a.h) + (row + AHEAD * step) * a.ld_h, a.dim * (int)sizeof(T));
+            look_ahead(static_cast<const T *>(a.dy) + (row + AHEAD * step) * a.ld_dy, a.dim * (int)sizeof(T));
+            if (a.dh)
+                look_ahead(static_cast<const T *>(a.dh) + (row + AHEAD * step) * a.ld_dh, a.dim * (int)sizeof(T));
+        }
         float n[VPT][VW], g[VPT][VW], dh[VPT][VW];
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
@@ -495,7 +544,7 @@ struct Backward {
 };
 
 // Fewest threads that hold a row in 16 values each (8 where they come singly, and less in narrow rows); false beyond 8,192 columns.
-// (More would spill beside 64-bit copies, fewer leave too few loads in flight.)
+// (More would spill beside the 8-bit form's second numbers, fewer leave too few loads in flight.)
 template <typename T, int VW, typename L> bool by_width(int dim, L l, cudaError_t &e)
 {
     const int nv = (dim + VW - 1) / VW;
