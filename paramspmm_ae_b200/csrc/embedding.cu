@@ -8,8 +8,10 @@
 // Runs that cross the border of a chunk leave their pieces in scratch, which a dependent launch adds in order: no atomics
 // on values, and the hottest id does not hold the launch up.  The rows that no id names are zeroed, with all others, by CTAs of the
 // sorting kernels, which leave the memory system idle.
-// Up to RANK_MAX ids are sorted by counting, one launch; more by least-significant-digit passes of up to 8 bits, as many as the
+// Up to RANK_MAX ids are sorted by counting, one launch; more by least-significant-digit passes of up to 9 bits, as many as the
 // table's size needs, one or two launches each: a pass counts the digits of the next one while it places its keys.
+// Lookup and gradient in us: 1,000,003 ids of 2,449,029 rows of 64 fp32 77 + 245, of which 90 write the zeros of dT; 32,768 ids into
+// 50,021 rows of 1,024 bf16 21 + 66; 200,003 ids into 100,003 rows of 47 fp32 17 + 53, of which 31 sort.
 // Ids outside the table: NaN rows in the lookup, nothing in the gradient, and pspmm_embedding_status tells.
 #include "feature_types.cuh"
 
@@ -21,6 +23,7 @@ __device__ unsigned g_embedding_status;
 constexpr int RANK_MAX = 2048;
 constexpr int TILE_THREADS = 256, TILE_KEYS = 8, TILE = TILE_THREADS * TILE_KEYS;  // keys of a CTA in a digit pass
 constexpr int WARPS = TILE_THREADS / 32;
+constexpr int DIGIT_BITS = 9, DIGITS = 1 << DIGIT_BITS;  // at most (nine: a table of 2^17 to 2^18 rows in two passes, not three)
 constexpr int SCAN_TILES = 32;
 constexpr int HOT = 64;  // chunks from which on a run's pieces are added by a CTA
 
@@ -52,7 +55,7 @@ struct SortArgs {
     const uint2 *from;  // null: the first pass, from `in`
     uint2 *to;
     uint32_t *counts;   // keys of each digit and tile; where scanned, each tile's first place inside its digit
-    uint32_t *totals;   // [256] of a scanned pass; null: the tiles add up the counts before them on their own
+    uint32_t *totals;   // [digits] of a scanned pass; null: the tiles add up the counts before them on their own
     uint32_t *next;     // counts of the next pass, added up while this one's keys are placed; null: there is none
     int32_t tiles, shift;
     int32_t passes, bits, mask;  // of a digit
@@ -173,7 +176,7 @@ __device__ __forceinline__ void fill_zeros(const Fill &f, int cta)
 // Counts lie by tile where the tiles read them all, else by digit.
 __device__ __forceinline__ int64_t count_at(const SortArgs &a, int64_t tile, uint32_t digit)
 {
-    return a.totals ? digit * (int64_t)a.tiles + tile : tile * 256 + digit;
+    return a.totals ? digit * (int64_t)a.tiles + tile : (tile << a.bits) + digit;
 }
 
 // Few ids: the place of a key is the number of smaller ones and of equal ones before it; a warp counts for one key.
@@ -209,15 +212,17 @@ __device__ __forceinline__ uint2 sort_pair(const SortArgs &a, int64_t i)
 // Of the first pass; the others are counted by the pass before.
 __global__ void __launch_bounds__(TILE_THREADS) digit_count_kernel(const SortArgs a)
 {
-    __shared__ uint32_t bins[256];
+    __shared__ uint32_t bins[DIGITS];
     pdl_launch_dependents();
     if ((int)blockIdx.x >= a.work) {
         fill_zeros(a.fill, blockIdx.x - a.work);
         return;
     }
-    bins[threadIdx.x] = 0;
-    for (int p = 1; p < a.passes; ++p)
-        a.counts[((int64_t)p * a.tiles + blockIdx.x) * 256 + threadIdx.x] = 0;
+    for (int d = threadIdx.x; d <= a.mask; d += TILE_THREADS) {
+        bins[d] = 0;
+        for (int p = 1; p < a.passes; ++p)
+            a.counts[(((int64_t)p * a.tiles + blockIdx.x) << a.bits) + d] = 0;
+    }
     __syncthreads();
     uint32_t key[TILE_KEYS];
 #pragma unroll
@@ -230,7 +235,8 @@ __global__ void __launch_bounds__(TILE_THREADS) digit_count_kernel(const SortArg
         if ((int64_t)blockIdx.x * TILE + k * TILE_THREADS + threadIdx.x < a.in.n)
             atomicAdd(&bins[key[k] >> a.shift & a.mask], 1u);
     __syncthreads();
-    a.counts[count_at(a, blockIdx.x, threadIdx.x)] = bins[threadIdx.x];
+    for (int d = threadIdx.x; d <= a.mask; d += TILE_THREADS)
+        a.counts[count_at(a, blockIdx.x, d)] = bins[d];
 }
 
 // Sum over the threads before this one, in a CTA of 256; `warps` is scratch of 8.
@@ -283,13 +289,16 @@ __global__ void __launch_bounds__(256) digit_scan_kernel(const SortArgs a)
         a.totals[blockIdx.x] = carry;
 }
 
-// Stable: a warp takes 256 neighbouring keys, 32 at a time; equal digits among the 32 find one another by a ballot per bit (a
-// third of what a match instruction takes), and a count per warp and digit carries on from one 32 to the next.  The tile is put in order in shared memory, so that equal digits leave
-// side by side.
+// Stable: a warp takes 256 neighbouring keys, 32 at a time; equal digits among the 32 find one another by a ballot per bit
+// (which was faster than one match instruction), and a count per warp and digit carries on from one 32 to the next.  The tile is put in
+// order in shared memory, so that equal digits leave side by side.  Bound by latency: 8 dependent rounds per warp, 10 to 17 us per pass of
+// 200,003 keys with its scan.
+// PER neighbouring digits per thread.
+template <int PER>
 __global__ void __launch_bounds__(TILE_THREADS) digit_scatter_kernel(const SortArgs a)
 {
-    __shared__ uint32_t seen[WARPS][256];
-    __shared__ uint32_t away[256];  // from a key's place in the tile to its place among all
+    __shared__ uint32_t seen[WARPS][256 * PER];
+    __shared__ uint32_t away[256 * PER];  // from a key's place in the tile to its place among all
     __shared__ uint32_t warps[8];
     __shared__ uint2 tile[TILE];
     pdl_launch_dependents();
@@ -298,8 +307,9 @@ __global__ void __launch_bounds__(TILE_THREADS) digit_scatter_kernel(const SortA
         return;
     }
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    for (int w = 0; w < WARPS; ++w)
-        seen[w][threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < WARPS * 256 * PER; i += TILE_THREADS)
+        (&seen[0][0])[i] = 0;
+    __syncthreads();
     pdl_wait();
     uint2 pair[TILE_KEYS];
     uint32_t rank[TILE_KEYS];
@@ -308,19 +318,26 @@ __global__ void __launch_bounds__(TILE_THREADS) digit_scatter_kernel(const SortA
     for (int k = 0; k < TILE_KEYS; ++k)
         if (i0 + k * 32 < a.in.n)
             pair[k] = sort_pair(a, i0 + k * 32);
-    uint32_t total, all = 0, earlier = 0;  // keys of this thread's digit: in all tiles, in those before this one
-    if (a.totals) {
-        all = a.totals[threadIdx.x];
-        earlier = a.counts[count_at(a, blockIdx.x, threadIdx.x)];
-    } else {
+    // keys of this thread's digits: in all tiles, in those before this one
+    uint32_t total, all[PER] = {}, earlier[PER] = {}, sum = 0;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int d = threadIdx.x * PER + e;
+        if (d > a.mask) {
+        } else if (a.totals) {
+            all[e] = a.totals[d];
+            earlier[e] = a.counts[count_at(a, blockIdx.x, d)];
+        } else {
 #pragma unroll 16
-        for (int t = 0; t < a.tiles; ++t) {
-            const uint32_t c = a.counts[t * 256 + threadIdx.x];
-            all += c;
-            earlier += t < (int)blockIdx.x ? c : 0;
+            for (int t = 0; t < a.tiles; ++t) {
+                const uint32_t c = a.counts[(t << a.bits) + d];
+                all[e] += c;
+                earlier[e] += t < (int)blockIdx.x ? c : 0;
+            }
         }
+        sum += all[e];
     }
-    const uint32_t first = exclusive_256(all, warps, total) + earlier;
+    uint32_t first = exclusive_256(sum, warps, total);
 #pragma unroll
     for (int k = 0; k < TILE_KEYS; ++k) {
         const bool in = i0 + k * 32 < a.in.n;
@@ -339,14 +356,21 @@ __global__ void __launch_bounds__(TILE_THREADS) digit_scatter_kernel(const SortA
     }
     __syncthreads();
     uint32_t mine = 0;
-    for (int w = 0; w < WARPS; ++w)
-        mine += seen[w][threadIdx.x];
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+        for (int w = 0; w < WARPS; ++w)
+            mine += seen[w][threadIdx.x * PER + e];
     uint32_t before = exclusive_256(mine, warps, total);
-    away[threadIdx.x] = first - before;
-    for (int w = 0; w < WARPS; ++w) {
-        const uint32_t c = seen[w][threadIdx.x];
-        seen[w][threadIdx.x] = before;
-        before += c;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int d = threadIdx.x * PER + e;
+        away[d] = first + earlier[e] - before;
+        first += all[e];
+        for (int w = 0; w < WARPS; ++w) {
+            const uint32_t c = seen[w][d];
+            seen[w][d] = before;
+            before += c;
+        }
     }
     __syncthreads();
 #pragma unroll
@@ -399,10 +423,10 @@ __device__ __forceinline__ int64_t warp_lower_bound(const uint2 *ids, uint32_t k
 }
 
 // A group of L lanes per chunk and slice of columns, a vector per lane, U rows in flight; a lane looks at a position, and the places of the
-// rows and of the runs' beginnings go round by shuffles and a ballot.  (Two or four vectors per lane and row: fewer groups and fewer rows
-// each; 32,768 rows of 1,024 bf16 31 us against 17.)
+// rows and of the runs' beginnings go round by shuffles and a ballot.  Bound by the latency of its gathers: 64 registers and 32 warps per SM were
+// faster than 80 and 24, spills and all (32,768 ids, rows of 1,024 bf16, sorting and all: 72 -> 67 us).
 template <typename T, int VW, int L>
-__global__ void __launch_bounds__(256, 3) grad_kernel(const GradArgs a)
+__global__ void __launch_bounds__(256, 4) grad_kernel(const GradArgs a)
 {
     constexpr int U = L < 8 ? L : sizeof(T) * VW <= 4 && L >= 16 ? 16 : 8;
     typedef Vec<T, VW> V;
@@ -613,8 +637,8 @@ GradScratch grad_scratch(int64_t n, int32_t dim)
     };
     for (int i = 0; i < 2; ++i)
         s.pairs[i] = take(i == 0 || n > RANK_MAX ? (size_t)n * 8 : 0);
-    s.counts = take(n > RANK_MAX ? 4 * tiles * 256 * 4 : 0);  // of up to four passes
-    s.totals = take(n > RANK_MAX ? 256 * 4 : 0);
+    s.counts = take(n > RANK_MAX ? 4 * tiles * DIGITS * 4 : 0);  // of up to four passes
+    s.totals = take(n > RANK_MAX ? DIGITS * 4 : 0);
     const int64_t run = run_for(n);
     s.part = take(n > run ? (size_t)((n + run - 1) / run) * 2 * (size_t)dim * 4 : 0);
     s.bytes = at;
@@ -720,8 +744,8 @@ extern "C" int pspmm_embedding_grad(const void *ids, int32_t ids64, int64_t n, c
     int bits = 1;
     while (bits < 32 && (n_rows >> bits) != 0)
         ++bits;  // keys are 0 .. n_rows
-    const int passes = n <= RANK_MAX ? 0 : (bits + 7) / 8, digit = passes ? (bits + passes - 1) / passes : 0;
-    // The counts before a tile: read by each up to this many tiles (tiles^2 KB in all), else scanned by a launch of its own.
+    const int passes = n <= RANK_MAX ? 0 : (bits + DIGIT_BITS - 1) / DIGIT_BITS, digit = passes ? (bits + passes - 1) / passes : 0;
+    // The counts before a tile: read by each up to this many tiles (tiles^2 or twice as many KB in all), else scanned by a launch of its own.
     const bool scan = tiles > SCAN_TILES;
     SortArgs s = {{ids, n, n_rows, padding, ids64 != 0}, nullptr, pairs[0], counts, scan ? (uint32_t *)(base + lay.totals) : nullptr,
                   nullptr, tiles, 0, passes, digit, (1 << digit) - 1, 0, {}};
@@ -754,11 +778,11 @@ extern "C" int pspmm_embedding_grad(const void *ids, int32_t ids64, int64_t n, c
         last = p ? last ^ 1 : 0;
         s.to = pairs[last];
         s.shift = digit * p;
-        s.counts = counts + (int64_t)p * tiles * 256;
-        s.next = p + 1 < passes ? s.counts + (int64_t)tiles * 256 : nullptr;
+        s.counts = counts + ((int64_t)p * tiles << digit);
+        s.next = p + 1 < passes ? s.counts + ((int64_t)tiles << digit) : nullptr;
         if (scan)
-            PSPMM_CUDA_TRY(then(digit_scan_kernel, 256, 1));
-        PSPMM_CUDA_TRY(then(digit_scatter_kernel, tiles, 2));
+            PSPMM_CUDA_TRY(then(digit_scan_kernel, 1 << digit, 1));
+        PSPMM_CUDA_TRY(then(digit > 8 ? digit_scatter_kernel<2> : digit_scatter_kernel<1>, tiles, 2));
     }
     const GradArgs a = {pairs[last], grad, out, (float *)(base + lay.part), n, n_rows, ld_grad, ld_out, 0, run_for(n), 0, 0, dim, 0, scale};
     PSPMM_CUDA_TRY(dtype == PSPMM_F32    ? grad_typed<float>(a, dim, st)

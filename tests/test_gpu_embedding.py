@@ -97,11 +97,11 @@ def test_one_id_takes_everything(n):
         check_grad(ids.flip(0).contiguous(), G, V)
 
 
-@pytest.mark.parametrize("V", [1, 2, 255, 256, 257, 65535, 65536, 65537, 16777215, 16777217])
-def test_table_sizes(V):
-    """Keys of one to four passes, the last id among them."""
+@pytest.mark.parametrize("V", [1, 2, 255, 256, 257, 511, 512, 65535, 65536, 65537, 131072, 262143, 262144, 16777217])
+@pytest.mark.parametrize("n", [3001, 70001])
+def test_table_sizes(V, n):
+    """Keys of one to three passes of every width, the last id among them, with few tiles of keys and with many."""
     g = torch.Generator().manual_seed(V)
-    n = 3001
     ids = (torch.rand(n, generator=g, dtype=torch.float64) * V).long().clamp_(max=V - 1)
     ids[:4] = V - 1
     G = torch.randint(-4, 5, (n, 4), generator=g).float()
@@ -111,6 +111,19 @@ def test_table_sizes(V):
     assert torch.equal(got.cpu(), want)
     ids = ids[:1000]
     assert torch.equal(fo.embedding_grad(ids.cuda(), G[:1000].cuda(), V).cpu(), torch.zeros(V, 4).index_add_(0, ids, G[:1000]))
+
+
+@pytest.mark.parametrize("n", [3001, 70001])
+def test_a_table_of_four_passes(n):
+    from paramspmm_ae_b200 import feature_ops as fo
+    V = 2 ** 27 + 1
+    g = torch.Generator().manual_seed(n)
+    ids = (torch.rand(n, generator=g, dtype=torch.float64) * V).long().clamp_(max=V - 1).cuda()
+    ids[:4] = V - 1
+    G = torch.randint(1, 5, (n, 1), generator=g).float().cuda()
+    got = fo.embedding_grad(ids, G, V)
+    want = torch.zeros(V, 1, device="cuda").index_add_(0, ids, G)  # whole numbers: any order is exact
+    assert torch.equal(got, want)
 
 
 def test_padding_no_ids_no_rows():
