@@ -21,58 +21,78 @@ struct Rows8Args {
     int32_t dim, pitch, blocks;
 };
 
-// LANES lanes share a block; each holds NV vectors of VW neighbouring columns, LANES * VW apart.  VW < 4: the lane's
-// four neighbouring columns come by loads of single values (rows that are not aligned), so that bytes leave as words.
-template <typename T, int VW> struct Shape {
-    static constexpr int COLS = VW < 4 ? 4 : VW;      // neighbouring columns of a lane
-    static constexpr int LANES = VW < 4 ? 32 : 8;
-    static constexpr int NV = EIGHT_BLOCK / (LANES * COLS);
+// LANES lanes share a block; each holds NV vectors of VW neighbouring columns, LANES * VW apart.  VW = 1, rows that are not aligned:
+// a warp's loads and its bytes lie side by side all the same, and 8 or 16 lanes do where the whole row is that narrow.
+template <int VW, int NARROW> struct Shape {
+    static constexpr int LANES = VW > 1 ? 8 : NARROW;
+    static constexpr int NV = VW > 1 ? EIGHT_BLOCK / (LANES * VW) : 4;
 };
 
-template <typename T, int VW>
-__device__ __forceinline__ void load_cols(float (&f)[Shape<T, VW>::COLS], const T *p, int left)
+// Unit (a row's block) of a lane group: 32-bit division where the count admits it (64-bit division was half of the odd widths' instructions).
+__device__ __forceinline__ int64_t unit_row(const Rows8Args &a, int64_t unit, int &block)
 {
-    constexpr int COLS = Shape<T, VW>::COLS;
-    if constexpr (VW < 4) {
-#pragma unroll
-        for (int i = 0; i < COLS; ++i)
-            f[i] = i < left ? to_float(p[i]) : 0.f;
-    } else {
-        if (left > 0) {  // (a whole vector: dim is a multiple of VW)
-            load_vec<T, VW>(f, p);
-        } else {
-#pragma unroll
-            for (int i = 0; i < COLS; ++i)
-                f[i] = 0.f;
-        }
+    if (a.blocks == 1) {
+        block = 0;
+        return unit;
     }
+    if (a.units <= UINT32_MAX) {
+        const uint32_t row = (uint32_t)unit / (uint32_t)a.blocks;
+        block = (int)((uint32_t)unit - row * (uint32_t)a.blocks);
+        return row;
+    }
+    const int64_t row = unit / a.blocks;
+    block = (int)(unit - row * a.blocks);
+    return row;
 }
 
-template <typename T, int VW>
+template <int VW> __device__ __forceinline__ void store_bytes(int8_t *q, const uint32_t (&b)[VW])
+{
+    if constexpr (VW == 8)
+        *reinterpret_cast<uint2 *>(q) = make_uint2(pack_bytes(b[0], b[1], b[2], b[3]), pack_bytes(b[4], b[5], b[6], b[7]));
+    else if constexpr (VW == 4)
+        *reinterpret_cast<uint32_t *>(q) = pack_bytes(b[0], b[1], b[2], b[3]);
+    else
+        *q = (int8_t)b[0];
+}
+
+template <typename T, int VW, int NARROW>
 __global__ void __launch_bounds__(256) quantize_kernel(const Rows8Args a)
 {
-    using S = Shape<T, VW>;
+    using S = Shape<VW, NARROW>;
     const int lane = threadIdx.x % S::LANES;
     const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / S::LANES;
     if (unit >= a.units)
         return;
-    const int64_t row = unit / a.blocks;
-    const int c0 = (int)(unit % a.blocks) * EIGHT_BLOCK + lane * S::COLS;
+    int block;
+    const int64_t row = unit_row(a, unit, block);
+    const int c0 = block * EIGHT_BLOCK + lane * VW;
     const T *x = static_cast<const T *>(a.x) + row * a.ld;
-    float f[S::NV][S::COLS];
+    float f[S::NV][VW];
 #pragma unroll
-    for (int v = 0; v < S::NV; ++v)
-        load_cols<T, VW>(f[v], x + c0 + v * S::LANES * S::COLS, a.dim - (c0 + v * S::LANES * S::COLS));
+    for (int v = 0; v < S::NV; ++v) {
+        const int c = c0 + v * S::LANES * VW;
+        if (c < a.dim) {  // (a whole vector: dim is a multiple of VW)
+            load_vec<T, VW>(f[v], x + c);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VW; ++i)
+                f[v][i] = 0.f;
+        }
+    }
     uint32_t top = 0;
 #pragma unroll
     for (int v = 0; v < S::NV; ++v)
 #pragma unroll
-        for (int i = 0; i < S::COLS; ++i)
+        for (int i = 0; i < VW; ++i)
             top = max(top, __float_as_uint(f[v][i]) & 0x7fffffffu);
     const uint32_t mask = S::LANES == 32 ? PSPMM_FULL_MASK : ((1u << S::LANES) - 1) << (threadIdx.x % 32 / S::LANES * S::LANES);
+    if constexpr (S::LANES == 32) {
+        top = __reduce_max_sync(mask, top);
+    } else {
 #pragma unroll
-    for (int d = S::LANES / 2; d > 0; d >>= 1)
-        top = max(top, __shfl_xor_sync(mask, top, d));
+        for (int d = S::LANES / 2; d > 0; d >>= 1)
+            top = max(top, __shfl_xor_sync(mask, top, d));
+    }
     float scale, up;
     eight_scale(top, scale, up);
     if (lane == 0)
@@ -80,78 +100,67 @@ __global__ void __launch_bounds__(256) quantize_kernel(const Rows8Args a)
     int8_t *q = a.q + row * a.pitch;
 #pragma unroll
     for (int v = 0; v < S::NV; ++v) {
-        const int c = c0 + v * S::LANES * S::COLS;
+        const int c = c0 + v * S::LANES * VW;
         if (c >= a.pitch)  // (the pitch is a multiple of 16; columns between dim and it are zeros)
             break;
-        uint32_t w[S::COLS / 4];
+        uint32_t b[VW];
 #pragma unroll
-        for (int i = 0; i < S::COLS / 4; ++i) {
-            uint32_t b[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                b[j] = eight_round(f[v][4 * i + j], up);
-            w[i] = pack_bytes(b[0], b[1], b[2], b[3]);
-        }
-        if constexpr (S::COLS == 8)
-            *reinterpret_cast<uint2 *>(q + c) = make_uint2(w[0], w[1]);
-        else
-            *reinterpret_cast<uint32_t *>(q + c) = w[0];
+        for (int i = 0; i < VW; ++i)
+            b[i] = eight_round(f[v][i], up);
+        store_bytes<VW>(q + c, b);
     }
 }
 
-template <typename T, int VW>
+template <typename T, int VW, int NARROW>
 __global__ void __launch_bounds__(256) dequantize_kernel(const Rows8Args a)
 {
-    using S = Shape<T, VW>;
+    using S = Shape<VW, NARROW>;
     const int lane = threadIdx.x % S::LANES;
     const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / S::LANES;
     if (unit >= a.units)
         return;
-    const int64_t row = unit / a.blocks;
-    const int c0 = (int)(unit % a.blocks) * EIGHT_BLOCK + lane * S::COLS;
+    int block;
+    const int64_t row = unit_row(a, unit, block);
+    const int c0 = block * EIGHT_BLOCK + lane * VW;
     const float scale = a.scales[unit];
     const int8_t *q = a.q + row * a.pitch;
     T *out = static_cast<T *>(const_cast<void *>(a.x)) + row * a.ld;
-    uint32_t w[S::NV][S::COLS / 4] = {};
+    uint32_t w[S::NV][(VW + 3) / 4] = {};
 #pragma unroll
     for (int v = 0; v < S::NV; ++v) {
-        const int c = c0 + v * S::LANES * S::COLS;
-        if (c < a.pitch) {
-            if constexpr (S::COLS == 8) {
+        const int c = c0 + v * S::LANES * VW;
+        if (c < a.dim) {
+            if constexpr (VW == 8) {
                 const uint2 u = *reinterpret_cast<const uint2 *>(q + c);
                 w[v][0] = u.x;
                 w[v][1] = u.y;
-            } else {
+            } else if constexpr (VW == 4) {
                 w[v][0] = *reinterpret_cast<const uint32_t *>(q + c);
+            } else {
+                w[v][0] = *reinterpret_cast<const uint8_t *>(q + c);
             }
         }
     }
 #pragma unroll
     for (int v = 0; v < S::NV; ++v) {
-        const int c = c0 + v * S::LANES * S::COLS;
-        float f[S::COLS];
+        const int c = c0 + v * S::LANES * VW;
+        float f[VW];
 #pragma unroll
-        for (int i = 0; i < S::COLS; ++i)
+        for (int i = 0; i < VW; ++i)
             f[i] = (float)(int8_t)(w[v][i / 4] >> (8 * (i % 4))) * scale;
-        if constexpr (VW < 4) {
-#pragma unroll
-            for (int i = 0; i < S::COLS; ++i)
-                if (c + i < a.dim)
-                    out[c + i] = from_float<T>(f[i]);
-        } else if (c < a.dim) {
+        if (c < a.dim)
             store_vec<T, VW>(out + c, f);
-        }
     }
 }
 
-template <typename T, int VW>
+template <typename T, int VW, int NARROW = 32>
 cudaError_t launch(bool quantize, const Rows8Args &a, cudaStream_t st)
 {
-    const int64_t ctas = (a.units * Shape<T, VW>::LANES + 255) / 256;
+    const int64_t ctas = (a.units * Shape<VW, NARROW>::LANES + 255) / 256;
     if (quantize)
-        quantize_kernel<T, VW><<<(unsigned)ctas, 256, 0, st>>>(a);
+        quantize_kernel<T, VW, NARROW><<<(unsigned)ctas, 256, 0, st>>>(a);
     else
-        dequantize_kernel<T, VW><<<(unsigned)ctas, 256, 0, st>>>(a);
+        dequantize_kernel<T, VW, NARROW><<<(unsigned)ctas, 256, 0, st>>>(a);
     return cudaGetLastError();
 }
 
@@ -165,7 +174,9 @@ cudaError_t launch_typed(bool quantize, const Rows8Args &a, cudaStream_t st)
     if constexpr (sizeof(T) == 2)
         if (a.dim % 4 == 0 && rows_aligned(a.x, a.ld, sizeof(T), 8))
             return launch<T, 4>(quantize, a, st);
-    return launch<T, 1>(quantize, a, st);
+    return a.dim <= 32   ? launch<T, 1, 8>(quantize, a, st)
+           : a.dim <= 64 ? launch<T, 1, 16>(quantize, a, st)
+                         : launch<T, 1>(quantize, a, st);
 }
 
 int rows8_run(bool quantize, const void *x, int32_t dtype, int64_t ld, int64_t n, int32_t dim, int8_t *q, int64_t pitch,
