@@ -4,17 +4,19 @@
 // and, where asked for, y in 8 bits (rows8.cu's form) from the same pass.
 //
 // Bound by HBM: every array is moved once.  A row is held in the registers of its lanes between the sum and its use: 8, 16 or
-// 32 lanes (several rows per warp) with up to 16 values each, a CTA of 64 to 1,024 threads beyond that, and two passes over a row
-// wider than 8,192 columns.  Rows of a CTA wait at a barrier between their sum and its use, so each asks for the row after the next
-// to be brought to L2.  x + r -> h, y in us (TB/s), alone, with y in 8 bits beside, and backward: 169,343 x 128 fp32
-// 66 (5.3), 72, 64; 16,384 x 4,096 bf16 120 (4.5), 217, 104; single values, 30,000 x 2,047 fp32 221 (4.4), 538, 193.  The 8-bit forms of
-// wide rows are bound by the instructions of the second number.  Rows brought to shared memory by bulk copies, several
-// in flight per CTA, were slower but for those (bf16 127, 210, 159): one more pass of instructions over every value.
+// 32 lanes (several rows per warp) with up to 16 values each, a CTA of as many warps as the row needs beyond that, and two passes over a
+// row wider than 8,192 columns.  Rows of a CTA wait at a barrier between their sum and its use, so each asks for the row after the next
+// to be brought to L2.  x + r -> h, y in us (TB/s), alone, with y in 8 bits beside, and backward: 169,343 x 128 fp32 61 (5.6), 70, 61;
+// 16,384 x 4,096 bf16 102 (5.2), 190, 102; single values, 30,000 x 2,047 fp32 186 (5.3), 225, 186.  The 8-bit forms of
+// wide rows are bound by the instructions of the second number.  (Measured and left: rows brought to shared memory by bulk copies, several in
+// flight per CTA, one more pass of instructions over every value, bf16 127, 210, 159; second numbers for the values next to a half
+// and the largest ones alone, from memory again, 190 -> 223.)
 //
-// Numbers: h = x + r is squared and added in 64 bits; rstd is kept in 32 bits for the backward, whose sums are in 32 bits.  y in 8 bits is
-// taken from a y with twice the bits of a 32-bit one, because next to a half the last bit of that decides which whole number it becomes;
-// y itself is the 32-bit one with and without it.  Those bits are a second 32-bit number (values below 1e-30 have fewer): in 64-bit
-// numbers the norm of 169,343 x 128 took 92 us against 66, most of it conversions, of which an SM does 16 per clock.
+// Numbers: the sum of h^2 has the bits of a 64-bit one but for what a 32-bit sum of 2^-24 of it loses; rstd is kept in 32 bits for the
+// backward, whose sums are in 32 bits.  y in 8 bits is taken from a y with twice the bits of a 32-bit one, because next to a half the last bit
+// of that decides which whole number it becomes; y itself is the 32-bit one with and without it.  Those bits are a second
+// 32-bit number (values below 1e-30 have fewer): in 64-bit numbers the norm of 169,343 x 128 took 92 us, most of it conversions, of
+// which an SM does 16 per clock.
 #include "feature_types.cuh"
 
 namespace {
@@ -48,11 +50,11 @@ struct WeightArgs {
 
 constexpr int AHEAD = 2;  // rows of a lane group that are brought to L2
 
-// TPR threads share a row; each holds VPT vectors of VW values.
+// TPR threads share a row; each holds VPT vectors of VW values.  TPR > 32: a CTA's threads, as many warps of the TPR / 32 as the row needs.
 template <int TPR> struct Rows {
-    static constexpr int THREADS = TPR <= 32 ? 256 : TPR;
-    static constexpr int PER_CTA = THREADS / TPR;
-    static constexpr int LANES = TPR < 32 ? TPR : 32;  // of a warp that share a row
+    static constexpr int MOST = TPR <= 32 ? 256 : TPR;  // threads of a CTA
+    static constexpr int PER_CTA = TPR <= 32 ? 256 / TPR : 1;
+    static constexpr int LANES = TPR <= 32 ? TPR : 32;  // of a warp that share a row
 };
 
 // Column of a thread's vector v: a warp's lanes side by side, a warp's vectors behind one another (so that the 128 columns of
@@ -82,19 +84,33 @@ template <typename S, int LANES> __device__ __forceinline__ S lanes_sum(S v, uin
     return v;
 }
 
-// Sum over a row's threads; `sums` has a place per warp and is used again from call to call (two barriers).
-template <typename S, int TPR> __device__ __forceinline__ S row_sum(S v, uint32_t mask, S *sums)
+// Sums of a CTA's warps: two sets in turn, so that a row needs one barrier (the next row's sums leave this row's alone, and the one
+// after that begins behind the next row's barrier).  What no warp writes stays 0.
+template <typename S, int WARPS> struct WarpSums {
+    S set[2][WARPS];
+    __device__ __forceinline__ void clear()
+    {
+        for (int i = threadIdx.x; i < (int)(sizeof(set) / sizeof(S)); i += blockDim.x)
+            set[0][i] = 0;
+        __syncthreads();
+    }
+};
+
+// Sum over a row's threads; `turn` alternates from row to row.
+template <typename S, int TPR, int WARPS> __device__ __forceinline__ S row_sum(S v, uint32_t mask, WarpSums<S, WARPS> &sums, int &turn)
 {
     v = lanes_sum<S, Rows<TPR>::LANES>(v, mask);
     if constexpr (TPR > 32) {
-        __syncthreads();
+        S *set = sums.set[turn];
+        turn ^= 1;
         if (threadIdx.x % 32 == 0)
-            sums[threadIdx.x / 32] = v;
+            set[threadIdx.x / 32] = v;
         __syncthreads();
-        v = 0;
+        S p[4] = {};
 #pragma unroll
-        for (int i = 0; i < TPR / 32; ++i)
-            v += sums[i];
+        for (int i = 0; i < WARPS; ++i)
+            p[i % 4] += set[i];
+        v = (p[0] + p[1]) + (p[2] + p[3]);
     }
     return v;
 }
@@ -126,11 +142,14 @@ __device__ __forceinline__ void look_ahead(const void *row, int bytes)
 }
 
 template <typename T, int VW, int TPR, int VPT, bool EIGHT>
-__global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs a)
+__global__ void __launch_bounds__(Rows<TPR>::MOST) norm_kernel(const NormArgs a)
 {
     using R = Rows<TPR>;
-    __shared__ double sums[R::THREADS / 32];
-    const int t = threadIdx.x % TPR;
+    __shared__ __align__(16) WarpSums<double, R::MOST / 32> sums;
+    int turn = 0;
+    if (TPR > 32)
+        sums.clear();
+    const int t = TPR > 32 ? threadIdx.x : threadIdx.x % R::LANES;
     const uint32_t mask = group_mask(R::LANES);
     float w[VPT][VW];
 #pragma unroll
@@ -139,7 +158,7 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs
         load_some<T, VW>(w[v], static_cast<const T *>(a.w) + c, c < a.dim);
     }
     const int64_t step = (int64_t)gridDim.x * R::PER_CTA;
-    for (int64_t row = (int64_t)blockIdx.x * R::PER_CTA + threadIdx.x / TPR; row < a.n; row += step) {
+    for (int64_t row = (int64_t)blockIdx.x * R::PER_CTA + (TPR > 32 ? 0 : threadIdx.x / R::LANES); row < a.n; row += step) {
         float h[VPT][VW], low[VPT][VW];  // x + r in 32 bits, and what that leaves of the residual until it is added
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
@@ -158,25 +177,35 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs
             if (a.r)
                 look_ahead(static_cast<const T *>(a.r) + (row + AHEAD * step) * a.ld_r, a.dim * (int)sizeof(T));
         }
+        // The sum of (h + low)^2, h = x + r rounded and low the exact remainder (Knuth's): h^2 in 64 bits and h low, 2^-24 of it, in 32.  (Both
+        // addends in 64 bits: two conversions per value, of which an SM does 16 per clock; 16,384 x 4,096 bf16 116 us against 102.)
         double ss = 0;
+        float cross = 0;
 #pragma unroll
         for (int v = 0; v < VPT; ++v)
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
                 if (a.r) {
-                    const double h64 = (double)h[v][i] + (double)low[v][i];
-                    ss = fma(h64, h64, ss);
                     const float x = h[v][i], r = low[v][i];
                     h[v][i] = x + r;
-                    if constexpr (EIGHT) {  // the exact remainder of a sum (Knuth's)
-                        const float b = h[v][i] - x;
-                        low[v][i] = (x - (h[v][i] - b)) + (r - b);
-                    }
+                    const float b = h[v][i] - x;
+                    low[v][i] = (x - (h[v][i] - b)) + (r - b);
+                    cross = fmaf(h[v][i], low[v][i], cross);
                 } else {
-                    ss = fma((double)h[v][i], (double)h[v][i], ss);
                     low[v][i] = 0.f;
                 }
+                ss = fma((double)h[v][i], (double)h[v][i], ss);
             }
+        if (fabsf(cross) < __int_as_float(0x7f800000)) {
+            ss = fma(2.0, (double)cross, ss);
+        } else {  // beyond the 32-bit numbers' range, or an infinity (whose remainder is none) or a NaN among the row
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int i = 0; i < VW; ++i)
+                    if (fabsf(low[v][i]) < __int_as_float(0x7f800000))
+                        ss = fma(2.0 * (double)h[v][i], (double)low[v][i], ss);
+        }
         if (a.h) {
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
@@ -185,7 +214,7 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs
                     store_vec<T, VW>(static_cast<T *>(a.h) + row * a.ld_h + c, h[v]);
             }
         }
-        ss = row_sum<double, TPR>(ss, mask, sums);
+        ss = row_sum<double, TPR>(ss, mask, sums, turn);
         const double rstd64 = inverse_root(ss / a.dim + a.eps);
         const float rstd = (float)rstd64;
         if (t == 0)
@@ -268,7 +297,9 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_kernel(const NormArgs
 template <typename T, bool EIGHT>
 __global__ void __launch_bounds__(1024) norm_wide_kernel(const NormArgs a)
 {
-    __shared__ double sums[32];
+    __shared__ __align__(16) WarpSums<double, 32> sums;
+    int turn = 0;
+    sums.clear();
     const T *w = static_cast<const T *>(a.w);
     for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
         const T *x = static_cast<const T *>(a.x) + row * a.ld_x;
@@ -278,7 +309,7 @@ __global__ void __launch_bounds__(1024) norm_wide_kernel(const NormArgs a)
             const double h = r ? (double)to_float(x[c]) + (double)to_float(r[c]) : (double)to_float(x[c]);
             ss = fma(h, h, ss);
         }
-        ss = row_sum<double, 1024>(ss, PSPMM_FULL_MASK, sums);
+        ss = row_sum<double, 1024>(ss, PSPMM_FULL_MASK, sums, turn);
         const double rstd64 = inverse_root(ss / a.dim + a.eps);
         const float rstd = (float)rstd64;
         if (threadIdx.x == 0)
@@ -326,12 +357,15 @@ __global__ void __launch_bounds__(1024) norm_wide_kernel(const NormArgs a)
 }
 
 template <typename T, int VW, int TPR, int VPT>
-__global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_backward_kernel(const NormBackArgs a)
+__global__ void __launch_bounds__(Rows<TPR>::MOST) norm_backward_kernel(const NormBackArgs a)
 {
     using R = Rows<TPR>;
     extern __shared__ float warps_dw[];  // [warps][dim] where several rows share a CTA
-    __shared__ float sums[R::THREADS / 32];
-    const int t = threadIdx.x % TPR;
+    __shared__ __align__(16) WarpSums<float, R::MOST / 32> sums;
+    int turn = 0;
+    if (TPR > 32)
+        sums.clear();
+    const int t = TPR > 32 ? threadIdx.x : threadIdx.x % R::LANES;
     const uint32_t mask = group_mask(R::LANES);
     float w[VPT][VW], dw[VPT][VW] = {};
 #pragma unroll
@@ -340,7 +374,7 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_backward_kernel(const
         load_some<T, VW>(w[v], static_cast<const T *>(a.w) + c, c < a.dim);
     }
     const int64_t step = (int64_t)gridDim.x * R::PER_CTA;
-    for (int64_t row = (int64_t)blockIdx.x * R::PER_CTA + threadIdx.x / TPR; row < a.n; row += step) {
+    for (int64_t row = (int64_t)blockIdx.x * R::PER_CTA + (TPR > 32 ? 0 : threadIdx.x / R::LANES); row < a.n; row += step) {
         if (TPR > 32 && t == 0 && row + AHEAD * step < a.n) {
             look_ahead(static_cast<const T *>(a.h) + (row + AHEAD * step) * a.ld_h, a.dim * (int)sizeof(T));
             look_ahead(static_cast<const T *>(a.dy) + (row + AHEAD * step) * a.ld_dy, a.dim * (int)sizeof(T));
@@ -374,7 +408,7 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_backward_kernel(const
                 g[v][i] *= w[v][i];
                 s = fmaf(g[v][i], n[v][i], s);
             }
-        s = row_sum<float, TPR>(s, mask, sums) / a.dim;
+        s = row_sum<float, TPR>(s, mask, sums, turn) / a.dim;
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
             const int c = column<VW, TPR, VPT>(t, v);
@@ -405,9 +439,9 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_backward_kernel(const
 #pragma unroll
             for (int i = 0; i < VW; ++i)
 #pragma unroll
-                for (int d = 16; d >= TPR; d >>= 1)
+                for (int d = 16; d >= R::LANES; d >>= 1)
                     dw[v][i] += __shfl_xor_sync(PSPMM_FULL_MASK, dw[v][i], d);
-        if (threadIdx.x % 32 < TPR) {
+        if (threadIdx.x % 32 < R::LANES) {
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
                 const int c = column<VW, TPR, VPT>(t, v);
@@ -418,10 +452,10 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_backward_kernel(const
             }
         }
         __syncthreads();
-        for (int c = threadIdx.x; c < a.dim; c += R::THREADS) {
+        for (int c = threadIdx.x; c < a.dim; c += R::MOST) {
             float s = 0;
 #pragma unroll
-            for (int i = 0; i < R::THREADS / 32; ++i)
+            for (int i = 0; i < R::MOST / 32; ++i)
                 s += warps_dw[i * a.dim + c];
             part[c] = s;
         }
@@ -431,7 +465,9 @@ __global__ void __launch_bounds__(Rows<TPR>::THREADS) norm_backward_kernel(const
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_wide_backward_kernel(const NormBackArgs a)
 {
-    __shared__ float sums[32];
+    __shared__ __align__(16) WarpSums<float, 32> sums;
+    int turn = 0;
+    sums.clear();
     const T *w = static_cast<const T *>(a.w);
     float *part = a.part + (int64_t)blockIdx.x * a.dim;
     for (int c = threadIdx.x; c < a.dim; c += 1024)
@@ -448,7 +484,7 @@ __global__ void __launch_bounds__(1024) norm_wide_backward_kernel(const NormBack
             part[c] = fmaf(g, n, part[c]);  // (a thread meets its own columns only)
             s = fmaf(g * to_float(w[c]), n, s);
         }
-        s = row_sum<float, 1024>(s, PSPMM_FULL_MASK, sums) / a.dim;
+        s = row_sum<float, 1024>(s, PSPMM_FULL_MASK, sums, turn) / a.dim;
         for (int c = threadIdx.x; c < a.dim; c += 1024) {
             const float n = to_float(hp[c]) * rstd;
             float g = to_float(dy[c]) * to_float(w[c]);
@@ -501,17 +537,17 @@ template <typename K> unsigned resident_grid(K kern, int threads, size_t smem, i
     return (unsigned)(ctas < most ? ctas : most);
 }
 
-template <typename T, int VW, int TPR, int VPT> cudaError_t launch_forward(const NormArgs &a, cudaStream_t st)
+template <int VW, int TPR, int VPT> int threads_for(int dim)
 {
-    using R = Rows<TPR>;
-    const int64_t ctas = (a.n + R::PER_CTA - 1) / R::PER_CTA;
-    if (a.q) {
-        auto kern = norm_kernel<T, VW, TPR, VPT, true>;
-        kern<<<resident_grid(kern, R::THREADS, 0, ctas), R::THREADS, 0, st>>>(a);
-    } else {
-        auto kern = norm_kernel<T, VW, TPR, VPT, false>;
-        kern<<<resident_grid(kern, R::THREADS, 0, ctas), R::THREADS, 0, st>>>(a);
-    }
+    return TPR <= 32 ? 256 : (dim + 32 * VW * VPT - 1) / (32 * VW * VPT) * 32;
+}
+
+template <typename T, int VW, int TPR, int VPT, bool EIGHT> cudaError_t launch_forward(const NormArgs &a, cudaStream_t st)
+{
+    const int64_t ctas = (a.n + Rows<TPR>::PER_CTA - 1) / Rows<TPR>::PER_CTA;
+    const int threads = threads_for<VW, TPR, VPT>(a.dim);
+    auto kern = norm_kernel<T, VW, TPR, VPT, EIGHT>;
+    kern<<<resident_grid(kern, threads, 0, ctas), threads, 0, st>>>(a);
     return cudaGetLastError();
 }
 
@@ -523,18 +559,19 @@ template <typename T, int VW, int TPR, int VPT> cudaError_t launch_backward(cons
 {
     using R = Rows<TPR>;
     auto kern = norm_backward_kernel<T, VW, TPR, VPT>;
-    const size_t smem = TPR > 32 ? 0 : (size_t)(R::THREADS / 32) * a.dim * 4;  // (at most 8 x 512 columns: 16 KB)
+    const int threads = threads_for<VW, TPR, VPT>(a.dim);
+    const size_t smem = TPR > 32 ? 0 : (size_t)8 * a.dim * 4;  // (at most 8 x 512 columns: 16 KB)
     int64_t ctas = (a.n + R::PER_CTA - 1) / R::PER_CTA;
     ctas = ctas < most_parts(a.n) ? ctas : most_parts(a.n);
-    parts = resident_grid(kern, R::THREADS, smem, ctas);
-    kern<<<parts, R::THREADS, smem, st>>>(a);
+    parts = resident_grid(kern, threads, smem, ctas);
+    kern<<<parts, threads, smem, st>>>(a);
     return cudaGetLastError();
 }
 
-struct Forward {
+template <bool EIGHT> struct Forward {
     const NormArgs &a;
     cudaStream_t st;
-    template <typename T, int VW, int TPR, int VPT> cudaError_t run() { return launch_forward<T, VW, TPR, VPT>(a, st); }
+    template <typename T, int VW, int TPR, int VPT> cudaError_t run() { return launch_forward<T, VW, TPR, VPT, EIGHT>(a, st); }
 };
 struct Backward {
     const NormBackArgs &a;
@@ -581,7 +618,7 @@ template <typename T, int VW, typename L> bool by_width(int dim, L l, cudaError_
     return true;
 }
 
-template <typename T> cudaError_t forward_typed(const NormArgs &a, cudaStream_t st)
+template <typename T, bool EIGHT> cudaError_t forward_typed(const NormArgs &a, cudaStream_t st)
 {
     constexpr int B = sizeof(T), WIDE = 16 / B;
     auto aligned = [&](int bytes) {
@@ -589,7 +626,7 @@ template <typename T> cudaError_t forward_typed(const NormArgs &a, cudaStream_t 
                rows_aligned(a.h, a.ld_h, B, bytes) && rows_aligned(a.y, a.ld_y, B, bytes) && rows_aligned(a.w, 0, B, bytes);
     };
     cudaError_t e = cudaSuccess;
-    const Forward l = {a, st};
+    const Forward<EIGHT> l = {a, st};
     if (aligned(16) && by_width<T, WIDE>(a.dim, l, e))
         return e;
     if constexpr (B == 2)
@@ -598,11 +635,12 @@ template <typename T> cudaError_t forward_typed(const NormArgs &a, cudaStream_t 
     if (by_width<T, 1>(a.dim, l, e))
         return e;
     const unsigned grid = (unsigned)(a.n < 2 * pspmm_sm_count() ? a.n : 2 * pspmm_sm_count());
-    if (a.q)
-        norm_wide_kernel<T, true><<<grid, 1024, 0, st>>>(a);
-    else
-        norm_wide_kernel<T, false><<<grid, 1024, 0, st>>>(a);
+    norm_wide_kernel<T, EIGHT><<<grid, 1024, 0, st>>>(a);
     return cudaGetLastError();
+}
+template <typename T> cudaError_t forward_typed(const NormArgs &a, cudaStream_t st)
+{
+    return a.q ? forward_typed<T, true>(a, st) : forward_typed<T, false>(a, st);
 }
 
 template <typename T> cudaError_t backward_typed(const NormBackArgs &a, unsigned &parts, cudaStream_t st)

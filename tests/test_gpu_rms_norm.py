@@ -144,6 +144,31 @@ def test_rows_of_zeros_and_values_at_the_ends():
     assert torch.isnan(relu[3]).all() and (relu[5] >= 0).all()
 
 
+@pytest.mark.parametrize("dim", [64, 300, 1100, 4101])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_residuals_at_the_ends(dtype, dim):
+    """Sums whose squares and remainders leave 32 bits, infinities and NaN on either side of the addition."""
+    from paramspmm_ae_b200 import feature_ops as fo
+    x, r, w = inputs(8, dim, dtype, 21)
+    x[0] *= 1e25
+    r[1] *= 1e30
+    x[2], r[2] = x[2] * 1e28, r[2] * 1e21  # the remainders of a row, added up, leave 32 bits
+    x[3, 5] = r[4, 6] = float("inf")
+    r[5, 7] = float("nan")
+    x[6, 8], r[6, 8] = float("inf"), float("-inf")
+    y, h, rstd, kept = fo.rms_norm(x.cuda(), w.cuda(), r.cuda(), eight_bit=True)
+    h64, rstd64, y64 = formula(x, r, w, 1e-6, False)
+    rows = [0, 1, 2, 7]
+    close(y[rows], y64[rows], (5 * U + half(dtype)) * y64[rows].abs() + 1e-44)
+    close(rstd[rows], rstd64[rows].squeeze(-1), 2 * U * rstd64[rows].squeeze(-1))
+    check(fo.Rows8(kept.q[rows].contiguous(), kept.scales[rows].contiguous(), dim), y64[rows])
+    y, h = y.cpu(), h.cpu()
+    for row, c in ((3, 5), (4, 6)):
+        assert torch.isinf(h[row, c]) and rstd[row] == 0
+        assert torch.isnan(y[row, c]) and not y[row, c + 1:].any()
+    assert torch.isnan(y[5:7]).all() and torch.isnan(rstd[5:7]).all()
+
+
 def backward_formula(dy, h, rstd, w, dh, relu):
     h, w, rstd = h.double(), w.double(), rstd.double().unsqueeze(-1)
     m = h * rstd
