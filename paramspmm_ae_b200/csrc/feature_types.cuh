@@ -42,6 +42,14 @@ template <typename T, int VW> __device__ __forceinline__ void store_vec(T *p, co
     *reinterpret_cast<Vec<T, VW> *>(p) = u;
 }
 
+// The larger one; NaN where either is.
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 // Scale of a block and the factor that takes its values to whole numbers, from the bits of its largest magnitude.  (As bits
 // a NaN is larger than an infinity is larger than any number, so one maximum of integers finds all three.)
 __device__ __forceinline__ void eight_scale(uint32_t top, float &scale, float &up)

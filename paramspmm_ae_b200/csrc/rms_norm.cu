@@ -6,8 +6,8 @@
 // Bound by HBM: every array is moved once.  A row is held in the registers of its lanes between the sum and its use: 8, 16 or
 // 32 lanes (several rows per warp) with up to 16 values each, a CTA of as many warps as the row needs beyond that, and two passes over a
 // row wider than 8,192 columns.  Rows of a CTA wait at a barrier between their sum and its use, so each asks for the row after the next
-// to be brought to L2.  x + r -> h, y in us (TB/s), alone, with y in 8 bits beside, and backward: 169,343 x 128 fp32 61 (5.6), 70, 61;
-// 16,384 x 4,096 bf16 102 (5.2), 190, 102; single values, 30,000 x 2,047 fp32 186 (5.3), 225, 186.  The 8-bit forms of
+// to be brought to L2.  x + r -> h, y in us (TB/s), alone, with y in 8 bits beside, and backward: 169,343 x 128 fp32 61 (5.6), 66, 62;
+// 16,384 x 4,096 bf16 92 (5.8), 167, 101; single values, 30,000 x 2,047 fp32 171 (5.7), 221, 185.  The 8-bit forms of
 // wide rows are bound by the instructions of the second number.  (Measured and left: rows brought to shared memory by bulk copies, several in
 // flight per CTA, one more pass of instructions over every value, bf16 127, 210, 159; second numbers for the values next to a half
 // and the largest ones alone, from memory again, 190 -> 223.)
@@ -141,8 +141,15 @@ __device__ __forceinline__ void look_ahead(const void *row, int bytes)
         asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"((uint32_t)(to - from)) : "memory");
 }
 
+// CTAs per SM that a kernel's registers leave room for (left to itself the compiler takes more registers than its loads repay in the lane
+// groups: 400,000 x 250 bf16 236 us against 205).
+constexpr int ctas_for(int tpr, int values, bool eight)
+{
+    return tpr > 32 ? 1 : values <= 4 ? 5 - eight : values <= 8 ? 4 - eight : 2;
+}
+
 template <typename T, int VW, int TPR, int VPT, bool EIGHT>
-__global__ void __launch_bounds__(Rows<TPR>::MOST) norm_kernel(const NormArgs a)
+__global__ void __launch_bounds__(Rows<TPR>::MOST, ctas_for(TPR, VW * VPT, EIGHT)) norm_kernel(const NormArgs a)
 {
     using R = Rows<TPR>;
     __shared__ __align__(16) WarpSums<double, R::MOST / 32> sums;
@@ -157,20 +164,30 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST) norm_kernel(const NormArgs a)
         const int c = column<VW, TPR, VPT>(t, v);
         load_some<T, VW>(w[v], static_cast<const T *>(a.w) + c, c < a.dim);
     }
+    const float least = a.relu ? 0.f : -__int_as_float(0x7f800000);
     const int64_t step = (int64_t)gridDim.x * R::PER_CTA;
     for (int64_t row = (int64_t)blockIdx.x * R::PER_CTA + (TPR > 32 ? 0 : threadIdx.x / R::LANES); row < a.n; row += step) {
+        // Without r, zeros are added all the same (16,384 x 4,096 bf16 102 us with a test per value, 92 without) but where
+        // registers are short and the test leaves more warps: 400,000 x 250 bf16 304 us against 215.
+        constexpr bool ALWAYS = VW > 1 || (TPR > 32 && TPR < 1024);
         float h[VPT][VW], low[VPT][VW];  // x + r in 32 bits, and what that leaves of the residual until it is added
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
             const int c = column<VW, TPR, VPT>(t, v);
             load_some<T, VW>(h[v], static_cast<const T *>(a.x) + row * a.ld_x + c, c < a.dim);
         }
-        if (a.r) {
+        if (VW > 1 || a.r) {
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
                 const int c = column<VW, TPR, VPT>(t, v);
-                load_some<T, VW>(low[v], static_cast<const T *>(a.r) + row * a.ld_r + c, c < a.dim);
+                load_some<T, VW>(low[v], static_cast<const T *>(a.r) + row * a.ld_r + c, a.r && c < a.dim);
             }
+        } else {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int i = 0; i < VW; ++i)
+                    low[v][i] = 0.f;
         }
         if (TPR > 32 && t == 0 && row + AHEAD * step < a.n) {
             look_ahead(static_cast<const T *>(a.x) + (row + AHEAD * step) * a.ld_x, a.dim * (int)sizeof(T));
@@ -185,14 +202,12 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST) norm_kernel(const NormArgs a)
         for (int v = 0; v < VPT; ++v)
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
-                if (a.r) {
+                if (ALWAYS || a.r) {
                     const float x = h[v][i], r = low[v][i];
                     h[v][i] = x + r;
                     const float b = h[v][i] - x;
                     low[v][i] = (x - (h[v][i] - b)) + (r - b);
                     cross = fmaf(h[v][i], low[v][i], cross);
-                } else {
-                    low[v][i] = 0.f;
                 }
                 ss = fma((double)h[v][i], (double)h[v][i], ss);
             }
@@ -225,11 +240,8 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST) norm_kernel(const NormArgs a)
                 const int c = column<VW, TPR, VPT>(t, v);
                 float y[VW];
 #pragma unroll
-                for (int i = 0; i < VW; ++i) {
-                    y[i] = h[v][i] * rstd * w[v][i];
-                    if (a.relu && y[i] < 0.f)
-                        y[i] = 0.f;
-                }
+                for (int i = 0; i < VW; ++i)
+                    y[i] = max_nan(h[v][i] * rstd * w[v][i], least);
                 if (c < a.dim)
                     store_vec<T, VW>(static_cast<T *>(a.y) + row * a.ld_y + c, y);
             }
@@ -247,7 +259,7 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST) norm_kernel(const NormArgs a)
                     const float ey = fmaf(en, w[v][i], fmaf(n, w[v][i], -y));
                     h[v][i] = y + ey;
                     low[v][i] = (y - h[v][i]) + ey;
-                    if (a.relu && h[v][i] < 0.f)
+                    if (h[v][i] < least)
                         h[v][i] = low[v][i] = 0.f;
                 }
             // A block is LB lanes wide and SB vectors deep.
@@ -257,12 +269,13 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST) norm_kernel(const NormArgs a)
             int8_t *q = a.q + row * a.pitch;
 #pragma unroll
             for (int v0 = 0; v0 < VPT; v0 += SB) {
-                uint32_t top = 0;
+                float most = 0.f;
 #pragma unroll
                 for (int v = v0; v < v0 + SB && v < VPT; ++v)
 #pragma unroll
                     for (int i = 0; i < VW; ++i)
-                        top = max(top, __float_as_uint(h[v][i]) & 0x7fffffffu);
+                        most = max_nan(most, fabsf(h[v][i]));
+                uint32_t top = __float_as_uint(most);
 #pragma unroll
                 for (int d = LB / 2; d > 0; d >>= 1)
                     top = max(top, __shfl_xor_sync(mask, top, d));

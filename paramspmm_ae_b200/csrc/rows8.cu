@@ -79,12 +79,13 @@ __global__ void __launch_bounds__(256) quantize_kernel(const Rows8Args a)
                 f[v][i] = 0.f;
         }
     }
-    uint32_t top = 0;
+    float most = 0.f;
 #pragma unroll
     for (int v = 0; v < S::NV; ++v)
 #pragma unroll
         for (int i = 0; i < VW; ++i)
-            top = max(top, __float_as_uint(f[v][i]) & 0x7fffffffu);
+            most = max_nan(most, fabsf(f[v][i]));
+    uint32_t top = __float_as_uint(most);
     const uint32_t mask = S::LANES == 32 ? PSPMM_FULL_MASK : ((1u << S::LANES) - 1) << (threadIdx.x % 32 / S::LANES * S::LANES);
     if constexpr (S::LANES == 32) {
         top = __reduce_max_sync(mask, top);
