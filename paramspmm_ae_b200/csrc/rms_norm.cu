@@ -31,6 +31,7 @@ struct NormArgs {
     int64_t n, ld_x, ld_r, ld_h, ld_y;
     double eps;
     int32_t dim, pitch, blocks, relu;
+    int32_t used;     // columns of q that are written: dim and the zeros to the next multiple of 16
 };
 
 struct NormBackArgs {
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST, ctas_for(TPR, VW * VPT, EIGHT
 #pragma unroll
                     for (int i = 0; i < VW; ++i)
                         b[i] = eight_round(h[v][i], low[v][i], up);
-                    if (c < a.pitch) {  // columns between dim and the pitch hold zeros
+                    if (c < a.used) {
                         if constexpr (VW == 8)
                             *reinterpret_cast<uint2 *>(q + c) =
                                 make_uint2(pack_bytes(b[0], b[1], b[2], b[3]), pack_bytes(b[4], b[5], b[6], b[7]));
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(1024) norm_wide_kernel(const NormArgs a)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     b[i] = eight_round(y64[i], (double)up);
-                if (c0 < a.pitch)
+                if (c0 < a.used)
                     *reinterpret_cast<uint32_t *>(a.q + row * a.pitch + c0) = pack_bytes(b[0], b[1], b[2], b[3]);
             }
         }
@@ -716,7 +717,7 @@ extern "C" int pspmm_rms_norm(const void *x, int64_t ld_x, const void *residual,
     if (pitch > INT32_MAX - 8192 || dim > INT32_MAX - 8192)
         return PSPMM_E_RANGE;
     const NormArgs a = {x, residual, weight, h, y, rstd, q, scales, n, ld_x, ld_residual, ld_h, ld_y, eps, dim,
-                        (int32_t)pitch, (dim + EIGHT_BLOCK - 1) / EIGHT_BLOCK, relu};
+                        (int32_t)pitch, (dim + EIGHT_BLOCK - 1) / EIGHT_BLOCK, relu, (dim + 15) / 16 * 16};
     cudaStream_t st = (cudaStream_t)stream;
     PSPMM_CUDA_TRY(dtype == PSPMM_F32    ? forward_typed<float>(a, st)
                    : dtype == PSPMM_BF16 ? forward_typed<bf16>(a, st)

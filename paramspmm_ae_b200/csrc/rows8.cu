@@ -20,6 +20,7 @@ struct Rows8Args {
     int64_t n, ld;
     int64_t units;   // n * blocks
     int32_t dim, pitch, blocks;
+    int32_t used;    // dim and the zeros to the next multiple of 16; bytes behind them belong to the caller
 };
 
 // LANES lanes share a block; each holds NV vectors of VW neighbouring columns, LANES * VW apart.  (Eight lanes where four do: 32,768 x 4,096
@@ -104,7 +105,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const Rows8Args a)
 #pragma unroll
     for (int v = 0; v < S::NV; ++v) {
         const int c = c0 + v * S::LANES * VW;
-        if (c >= a.pitch)  // (the pitch is a multiple of 16; columns between dim and it are zeros)
+        if (c >= a.used)
             break;
         uint32_t b[VW];
 #pragma unroll
@@ -192,11 +193,10 @@ int rows8_run(bool quantize, const void *x, int32_t dtype, int64_t ld, int64_t n
     if (!x || !q || !scales || (uintptr_t)q % 16 != 0 || (uintptr_t)scales % 4 != 0 || (uintptr_t)x % elem_bytes(dtype) != 0)
         return PSPMM_E_ARG;
     const int64_t blocks = ((int64_t)dim + EIGHT_BLOCK - 1) / EIGHT_BLOCK;
-    // (bytes of q between the last column's 16 and a longer pitch belong to the caller)
     const int64_t units = n * blocks;
-    if (pitch > INT32_MAX || n > ((int64_t)INT32_MAX * 8) / blocks)  // CTAs of eight blocks
+    if (pitch > INT32_MAX || dim > INT32_MAX - 8192 || n > ((int64_t)INT32_MAX * 8) / blocks)  // CTAs of eight blocks
         return PSPMM_E_RANGE;
-    Rows8Args a = {x, q, scales, n, ld, units, dim, (int32_t)pitch, (int32_t)blocks};
+    Rows8Args a = {x, q, scales, n, ld, units, dim, (int32_t)pitch, (int32_t)blocks, (dim + 15) / 16 * 16};
     cudaError_t e = dtype == PSPMM_F32    ? launch_typed<float>(quantize, a, (cudaStream_t)stream)
                     : dtype == PSPMM_BF16 ? launch_typed<bf16>(quantize, a, (cudaStream_t)stream)
                                           : launch_typed<f16>(quantize, a, (cudaStream_t)stream);

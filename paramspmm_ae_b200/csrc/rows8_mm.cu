@@ -680,7 +680,7 @@ int mm_run(const int8_t *q, int64_t pitch, const float *scales, int64_t rows, in
         return PSPMM_OK;
     if (!C || (uintptr_t)C % 4 != 0)
         return PSPMM_E_ARG;
-    if (dim > (1 << 20) || cols > (1 << 20))
+    if (dim > (1 << 20) || cols > (1 << 20) || (int64_t)dim * cols > (int64_t)INT32_MAX * 32)
         return PSPMM_E_RANGE;
     cudaStream_t st = (cudaStream_t)stream;
     if (rows == 0) {

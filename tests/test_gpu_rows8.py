@@ -1,5 +1,7 @@
 """Rows held in 8 bits, against the definition in 64 bits.  Whole numbers and scales have to be equal: a / 127 and 127 / a are
 single 32-bit divisions, and x * (127 / a) is exact in 64 bits before it is rounded."""
+import ctypes
+
 import pytest
 import torch
 
@@ -122,3 +124,30 @@ def test_more_than_two_to_the_31_values():
     check(part, x[rows.cuda()].float().cpu())
     out = kept.dequantize(torch.bfloat16)
     assert torch.equal(out[rows.cuda()], part.dequantize(torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [5, 40, 47, 144, 300, 1030, 9000])
+def test_a_longer_pitch_is_left_alone(pspmm_lib, dtype, dim):
+    """Through the C ABI: columns up to the next multiple of 16 become zeros, those behind them keep what they held."""
+    n, used = 9, dim + -dim % 16
+    pitch, t = used + 160, TYPES.index(dtype)
+    x = torch.randn(n, dim, generator=torch.Generator().manual_seed(dim)).to(dtype).cuda()
+    w = torch.ones(dim, dtype=dtype, device="cuda")
+    scales = torch.empty(n, (dim + BLOCK - 1) // BLOCK, device="cuda")
+    rstd = torch.empty(n, device="cuda")
+    ptr = lambda a: ctypes.c_void_p(a.data_ptr())
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for norm in (False, True):
+        q = torch.full((n, pitch), 77, dtype=torch.int8, device="cuda")
+        if norm:
+            rc = pspmm_lib.pspmm_rms_norm(ptr(x), dim, None, 0, ptr(w), t, n, dim, 1e-6, 0, None, dim, None, dim, ptr(rstd), ptr(q),
+                                          pitch, ptr(scales), stream)
+        else:
+            rc = pspmm_lib.pspmm_quantize_rows(ptr(x), t, dim, n, dim, ptr(q), pitch, ptr(scales), stream)
+        assert rc == 0
+        assert not q[:, dim:used].any() and (q[:, used:] == 77).all()
+        assert (q[:, :dim].abs().amax(1) == 127).all()
+        out = torch.empty(n, dim, device="cuda")
+        assert pspmm_lib.pspmm_dequantize_rows(ptr(q), pitch, ptr(scales), 0, ptr(out), dim, n, dim, stream) == 0
+        assert torch.equal(out, q[:, :dim].float() * scales.repeat_interleave(BLOCK, 1)[:, :dim])
