@@ -96,7 +96,7 @@ def embedding(ids, table, scale=1.0):
     if table.dim() != 2:
         raise RuntimeError("table must be 2-dimensional")
     rows, dim, ld = _rows(table, "table")
-    out = table.new_empty(ids.shape + (dim,))
+    out = table.new_empty((*ids.shape, dim))
     rc = lib().pspmm_embedding(ids.data_ptr(), wide, ids.numel(), table.data_ptr(), _DTYPES[table.dtype], rows, dim, ld, scale,
                                out.data_ptr(), dim, _stream())
     if rc:
