@@ -42,6 +42,40 @@ template <typename T, int VW> __device__ __forceinline__ void store_vec(T *p, co
     *reinterpret_cast<Vec<T, VW> *>(p) = u;
 }
 
+// Two floats side by side in 64 bits, for the packed instructions.
+typedef unsigned long long pair_t;
+__device__ __forceinline__ pair_t make_pair(float x0, float x1)
+{
+    pair_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x0), "f"(x1));
+    return p;
+}
+__device__ __forceinline__ void get_pair(pair_t p, float &x0, float &x1) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x0), "=f"(x1) : "l"(p)); }
+__device__ __forceinline__ pair_t add_pair(pair_t a, pair_t b)
+{
+    pair_t p;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+    return p;
+}
+__device__ __forceinline__ pair_t mul_pair(pair_t a, pair_t b)
+{
+    pair_t p;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+    return p;
+}
+__device__ __forceinline__ pair_t sub_pair(pair_t a, pair_t b)
+{
+    pair_t p;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+    return p;
+}
+__device__ __forceinline__ pair_t fma_pair(pair_t a, pair_t b, pair_t c)
+{
+    pair_t p;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(a), "l"(b), "l"(c));
+    return p;
+}
+
 // The larger one; NaN where either is.
 __device__ __forceinline__ float max_nan(float a, float b)
 {
@@ -71,8 +105,17 @@ __device__ __forceinline__ uint32_t eight_round(double x, double up)
 {
     return (uint32_t)__double2loint(fma(x, up, 6755399441055744.0));
 }
+// rint(x * up) from the rounded product, and how far that is from it: what a second number adds to x, 2^-24 of it at most, and the
+// product's rounding matter within NEAR_HALF of a half (127 2^-24 and 2^-18 together are a quarter of that).
+constexpr float NEAR_HALF = 0x1p-15f;
+__device__ __forceinline__ uint32_t eight_round(float x, float up, float &off)
+{
+    const float z = x * up, m = z + 12582912.f;
+    off = fabsf(z - (m - 12582912.f));
+    return __float_as_uint(m);
+}
 // The same for x + low, low what x's rounding left of it.
-__device__ __forceinline__ uint32_t eight_round(float x, float low, float up)
+__device__ __forceinline__ uint32_t eight_round_low(float x, float low, float up)
 {
     const float z = x * up, ez = fmaf(low, up, fmaf(x, up, -z));
     const float m = z + 12582912.f;

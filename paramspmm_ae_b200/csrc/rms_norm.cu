@@ -171,6 +171,11 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST, ctas_for(TPR, VW * VPT, EIGHT
         // Without r, zeros are added all the same (16,384 x 4,096 bf16 102 us with a test per value, 92 without) but where
         // registers are short and the test leaves more warps: 400,000 x 250 bf16 304 us against 215.
         constexpr bool ALWAYS = VW > 1 || (TPR > 32 && TPR < 1024);
+        constexpr int VALUES = VPT * VW;
+        static_assert(VALUES % 2 == 0, "values are worked on in pairs");
+        auto at = [](auto &m, int e) -> auto & { return m[e / VW][e % VW]; };
+        auto pair_of = [&](auto &m, int e) { return make_pair(at(m, e), at(m, e + 1)); };
+        auto set_pair = [&](auto &m, int e, pair_t p) { get_pair(p, at(m, e), at(m, e + 1)); };
         float h[VPT][VW], low[VPT][VW];  // x + r in 32 bits, and what that leaves of the residual until it is added
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
@@ -198,20 +203,22 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST, ctas_for(TPR, VW * VPT, EIGHT
         // The sum of (h + low)^2, h = x + r rounded and low the exact remainder (Knuth's): h^2 in 64 bits and h low, 2^-24 of it, in 32.  (Both
         // addends in 64 bits: two conversions per value, of which an SM does 16 per clock; 16,384 x 4,096 bf16 116 us against 102.)
         double ss = 0;
-        float cross = 0;
+        pair_t crosses = 0;
 #pragma unroll
-        for (int v = 0; v < VPT; ++v)
-#pragma unroll
-            for (int i = 0; i < VW; ++i) {
-                if (ALWAYS || a.r) {
-                    const float x = h[v][i], r = low[v][i];
-                    h[v][i] = x + r;
-                    const float b = h[v][i] - x;
-                    low[v][i] = (x - (h[v][i] - b)) + (r - b);
-                    cross = fmaf(h[v][i], low[v][i], cross);
-                }
-                ss = fma((double)h[v][i], (double)h[v][i], ss);
+        for (int e = 0; e < VALUES; e += 2) {
+            if (ALWAYS || a.r) {
+                const pair_t x = pair_of(h, e), r = pair_of(low, e), sum = add_pair(x, r), b = sub_pair(sum, x);
+                const pair_t rest = add_pair(sub_pair(x, sub_pair(sum, b)), sub_pair(r, b));
+                crosses = fma_pair(sum, rest, crosses);
+                set_pair(h, e, sum);
+                set_pair(low, e, rest);
             }
+            const double h0 = at(h, e), h1 = at(h, e + 1);
+            ss = fma(h1, h1, fma(h0, h0, ss));
+        }
+        float cross, cross1;
+        get_pair(crosses, cross, cross1);
+        cross += cross1;
         if (fabsf(cross) < __int_as_float(0x7f800000)) {
             ss = fma(2.0, (double)cross, ss);
         } else {  // beyond the 32-bit numbers' range, or an infinity (whose remainder is none) or a NaN among the row
@@ -240,9 +247,16 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST, ctas_for(TPR, VW * VPT, EIGHT
             for (int v = 0; v < VPT; ++v) {
                 const int c = column<VW, TPR, VPT>(t, v);
                 float y[VW];
+                if constexpr (VW == 1) {
+                    y[0] = max_nan(h[v][0] * rstd * w[v][0], least);
+                } else {
 #pragma unroll
-                for (int i = 0; i < VW; ++i)
-                    y[i] = max_nan(h[v][i] * rstd * w[v][i], least);
+                    for (int i = 0; i < VW; i += 2) {
+                        get_pair(mul_pair(mul_pair(pair_of(h, v * VW + i), make_pair(rstd, rstd)), pair_of(w, v * VW + i)), y[i], y[i + 1]);
+                        y[i] = max_nan(y[i], least);
+                        y[i + 1] = max_nan(y[i + 1], least);
+                    }
+                }
                 if (c < a.dim)
                     store_vec<T, VW>(static_cast<T *>(a.y) + row * a.ld_y + c, y);
             }
@@ -250,19 +264,18 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST, ctas_for(TPR, VW * VPT, EIGHT
         if constexpr (EIGHT) {
             // (h + low) rstd w as a sum of two 32-bit numbers, the first the sum rounded: products and what their rounding leaves (fma).
             const float rest = (float)(rstd64 - rstd);
+            const pair_t by = make_pair(rstd, rstd), by_less = make_pair(-rstd, -rstd), by_rest = make_pair(rest, rest);
 #pragma unroll
-            for (int v = 0; v < VPT; ++v)
-#pragma unroll
-                for (int i = 0; i < VW; ++i) {
-                    const float n = h[v][i] * rstd;
-                    const float en = fmaf(low[v][i], rstd, fmaf(h[v][i], rest, fmaf(h[v][i], rstd, -n)));
-                    const float y = n * w[v][i];
-                    const float ey = fmaf(en, w[v][i], fmaf(n, w[v][i], -y));
-                    h[v][i] = y + ey;
-                    low[v][i] = (y - h[v][i]) + ey;
-                    if (h[v][i] < least)
-                        h[v][i] = low[v][i] = 0.f;
-                }
+            for (int e = 0; e < VALUES; e += 2) {
+                const pair_t x = pair_of(h, e), f = pair_of(w, e), n = mul_pair(x, by), less_n = mul_pair(x, by_less);
+                const pair_t en = fma_pair(pair_of(low, e), by, fma_pair(x, by_rest, fma_pair(x, by, less_n)));
+                const pair_t less_y = mul_pair(less_n, f), ey = fma_pair(en, f, fma_pair(n, f, less_y));
+                const pair_t y = sub_pair(ey, less_y);
+                set_pair(low, e, sub_pair(ey, add_pair(less_y, y)));
+                set_pair(h, e, y);
+                at(h, e) = max_nan(at(h, e), least);  // (the second number of a value cut to 0 is not looked at)
+                at(h, e + 1) = max_nan(at(h, e + 1), least);
+            }
             // A block is LB lanes wide and SB vectors deep.
             constexpr int LB = R::LANES * VW >= EIGHT_BLOCK ? EIGHT_BLOCK / VW : R::LANES;
             constexpr int DEEP = EIGHT_BLOCK / (LB * VW), SB = DEEP < VPT ? DEEP : VPT;
@@ -289,9 +302,18 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST, ctas_for(TPR, VW * VPT, EIGHT
                 for (int v = v0; v < v0 + SB && v < VPT; ++v) {
                     const int c = column<VW, TPR, VPT>(t, v);
                     uint32_t b[VW];
+                    float off[VW], most_off = 0.f;  // (fmaxf leaves out the NaN of a block without a scale)
 #pragma unroll
-                    for (int i = 0; i < VW; ++i)
-                        b[i] = eight_round(h[v][i], low[v][i], up);
+                    for (int i = 0; i < VW; ++i) {
+                        b[i] = eight_round(h[v][i], up, off[i]);
+                        most_off = fmaxf(most_off, off[i]);
+                    }
+                    if (most_off > 0.5f - NEAR_HALF) {  // one value in 2^14
+#pragma unroll
+                        for (int i = 0; i < VW; ++i)
+                            if (off[i] > 0.5f - NEAR_HALF)
+                                b[i] = eight_round_low(h[v][i], low[v][i], up);
+                    }
                     if (c < a.used) {
                         if constexpr (VW == 8)
                             *reinterpret_cast<uint2 *>(q + c) =

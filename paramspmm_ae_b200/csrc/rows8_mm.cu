@@ -142,28 +142,6 @@ __device__ __forceinline__ uint32_t bf16_pair(uint32_t w, uint32_t pick)
     return *reinterpret_cast<const uint32_t *>(&d);
 }
 
-// Two floats side by side in 64 bits, for the packed instructions.
-typedef unsigned long long pair_t;
-__device__ __forceinline__ pair_t make_pair(float x0, float x1)
-{
-    pair_t p;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x0), "f"(x1));
-    return p;
-}
-__device__ __forceinline__ void get_pair(pair_t p, float &x0, float &x1) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x0), "=f"(x1) : "l"(p)); }
-__device__ __forceinline__ pair_t add_pair(pair_t a, pair_t b)
-{
-    pair_t p;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
-    return p;
-}
-__device__ __forceinline__ pair_t mul_pair(pair_t a, pair_t b)
-{
-    pair_t p;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
-    return p;
-}
-
 // The upper 16 bits of two values, cut off, as a bf16 pair; and what is left of the values.
 __device__ __forceinline__ uint32_t cut_pair(pair_t &x)
 {
