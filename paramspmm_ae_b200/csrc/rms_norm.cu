@@ -6,11 +6,11 @@
 // Bound by HBM: every array is moved once.  A row is held in the registers of its lanes between the sum and its use: 8, 16 or
 // 32 lanes (several rows per warp) with up to 16 values each, a CTA of as many warps as the row needs beyond that, and two passes over a
 // row wider than 8,192 columns.  Rows of a CTA wait at a barrier between their sum and its use, so each asks for the row after the next
-// to be brought to L2.  x + r -> h, y in us (TB/s), alone, with y in 8 bits beside, and backward: 169,343 x 128 fp32 61 (5.6), 66, 62;
-// 16,384 x 4,096 bf16 92 (5.8), 167, 101; single values, 30,000 x 2,047 fp32 171 (5.7), 221, 185.  The 8-bit forms of
-// wide rows are bound by the instructions of the second number.  (Measured and left: rows brought to shared memory by bulk copies, several in
+// to be brought to L2.  x + r -> h, y in us (TB/s), alone, with y in 8 bits beside, and backward: 169,343 x 128 fp32 60 (5.8), 64, 61;
+// 16,384 x 4,096 bf16 90 (6.0), 145, 105; single values, 30,000 x 2,047 fp32 172 (5.7), 219, 186, 400,000 x 250 bf16 201 (4.0), 344, 270.  The 8-bit forms of
+// wide rows are bound by instructions: 43 per value and thread, 56 % of issue slots.  (Measured and left: rows brought to shared memory by bulk copies, several in
 // flight per CTA, one more pass of instructions over every value, bf16 127, 210, 159; second numbers for the values next to a half
-// and the largest ones alone, from memory again, 190 -> 223.)
+// and the largest ones alone, from memory again, which was 15 % slower than all of them from registers.)
 //
 // Numbers: the sum of h^2 has the bits of a 64-bit one but for what a 32-bit sum of 2^-24 of it loses; rstd is kept in 32 bits for the
 // backward, whose sums are in 32 bits.  y in 8 bits is taken from a y with twice the bits of a 32-bit one, because next to a half the last bit
@@ -75,6 +75,14 @@ template <typename T, int VW> __device__ __forceinline__ void load_some(float (&
         for (int i = 0; i < VW; ++i)
             f[i] = 0.f;
     }
+}
+
+// A thread's values in pairs, for the packed instructions (half of what single ones take to issue).
+template <int N, int VW> __device__ __forceinline__ float &at(float (&m)[N][VW], int e) { return m[e / VW][e % VW]; }
+template <int N, int VW> __device__ __forceinline__ pair_t pair_of(float (&m)[N][VW], int e) { return make_pair(at(m, e), at(m, e + 1)); }
+template <int N, int VW> __device__ __forceinline__ void set_pair(float (&m)[N][VW], int e, pair_t p)
+{
+    get_pair(p, at(m, e), at(m, e + 1));
 }
 
 template <typename S, int LANES> __device__ __forceinline__ S lanes_sum(S v, uint32_t mask)
@@ -173,9 +181,6 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST, ctas_for(TPR, VW * VPT, EIGHT
         constexpr bool ALWAYS = VW > 1 || (TPR > 32 && TPR < 1024);
         constexpr int VALUES = VPT * VW;
         static_assert(VALUES % 2 == 0, "values are worked on in pairs");
-        auto at = [](auto &m, int e) -> auto & { return m[e / VW][e % VW]; };
-        auto pair_of = [&](auto &m, int e) { return make_pair(at(m, e), at(m, e + 1)); };
-        auto set_pair = [&](auto &m, int e, pair_t p) { get_pair(p, at(m, e), at(m, e + 1)); };
         float h[VPT][VW], low[VPT][VW];  // x + r in 32 bits, and what that leaves of the residual until it is added
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
@@ -432,31 +437,43 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST) norm_backward_kernel(const No
             }
         }
         const float rstd = a.rstd[row];
-        float s = 0;
+        const pair_t by = make_pair(rstd, rstd);
+        pair_t sum2 = 0;
 #pragma unroll
-        for (int v = 0; v < VPT; ++v)
-#pragma unroll
-            for (int i = 0; i < VW; ++i) {
-                n[v][i] *= rstd;
-                if (a.relu && !(n[v][i] * w[v][i] > 0.f))
-                    g[v][i] = 0.f;
-                dw[v][i] = fmaf(g[v][i], n[v][i], dw[v][i]);
-                g[v][i] *= w[v][i];
-                s = fmaf(g[v][i], n[v][i], s);
+        for (int e = 0; e < VPT * VW; e += 2) {
+            const pair_t m = mul_pair(pair_of(n, e), by), f = pair_of(w, e);
+            set_pair(n, e, m);
+            if (a.relu) {
+                float y0, y1;
+                get_pair(mul_pair(m, f), y0, y1);
+                if (!(y0 > 0.f))
+                    at(g, e) = 0.f;
+                if (!(y1 > 0.f))
+                    at(g, e + 1) = 0.f;
             }
-        s = row_sum<float, TPR>(s, mask, sums, turn) / a.dim;
+            set_pair(dw, e, fma_pair(pair_of(g, e), m, pair_of(dw, e)));
+            const pair_t gw = mul_pair(pair_of(g, e), f);
+            set_pair(g, e, gw);
+            sum2 = fma_pair(gw, m, sum2);
+        }
+        float s, s1;
+        get_pair(sum2, s, s1);
+        s = row_sum<float, TPR>(s + s1, mask, sums, turn) / a.dim;
+        const pair_t less_s = make_pair(-s, -s);
+#pragma unroll
+        for (int e = 0; e < VPT * VW; e += 2) {
+            const pair_t o = mul_pair(fma_pair(pair_of(n, e), less_s, pair_of(g, e)), by);
+            set_pair(g, e, o);
+            if (a.dh) {
+                at(g, e) += at(dh, e);
+                at(g, e + 1) += at(dh, e + 1);
+            }
+        }
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
             const int c = column<VW, TPR, VPT>(t, v);
-            float o[VW];
-#pragma unroll
-            for (int i = 0; i < VW; ++i) {
-                o[i] = (g[v][i] - n[v][i] * s) * rstd;
-                if (a.dh)
-                    o[i] += dh[v][i];
-            }
             if (c < a.dim)
-                store_vec<T, VW>(static_cast<T *>(a.dx) + row * a.ld_dx + c, o);
+                store_vec<T, VW>(static_cast<T *>(a.dx) + row * a.ld_dx + c, g[v]);
         }
     }
     float *part = a.part + (int64_t)blockIdx.x * a.dim;
