@@ -24,11 +24,12 @@ struct Rows8Args {
 };
 
 // LANES lanes share a block; each holds NV vectors of VW neighbouring columns, LANES * VW apart.  (Eight lanes where four do: 32,768 x 4,096
-// bf16 80 us against 70, the same divisions and shuffles for half the values.)  VW = 1, rows that are not aligned:
-// a warp's loads and its bytes lie side by side all the same, and 8 or 16 lanes do where the whole row is that narrow.
-template <int VW, int NARROW> struct Shape {
-    static constexpr int LANES = VW == 8 ? 4 : VW > 1 ? 8 : NARROW;
-    static constexpr int NV = VW > 1 ? EIGHT_BLOCK / (LANES * VW) : 4;
+// bf16 80 us against 70, the same divisions and shuffles for half the values.)  Rows of at most a quarter or a half of a block: CUT = 4
+// or 2, as many vectors fewer.  VW = 1, rows that are not aligned: a warp's loads and its bytes lie side by side all the same, and CUT times
+// fewer lanes do.
+template <int VW, int CUT> struct Shape {
+    static constexpr int LANES = VW == 8 ? 4 : VW > 1 ? 8 : 32 / CUT;
+    static constexpr int NV = VW > 1 ? EIGHT_BLOCK / (LANES * VW * CUT) : 4;
 };
 
 // Unit (a row's block) of a lane group: 32-bit division where the count admits it (64-bit division was half of the odd widths' instructions).
@@ -58,10 +59,10 @@ template <int VW> __device__ __forceinline__ void store_bytes(int8_t *q, const u
         *q = (int8_t)b[0];
 }
 
-template <typename T, int VW, int NARROW>
+template <typename T, int VW, int CUT>
 __global__ void __launch_bounds__(256) quantize_kernel(const Rows8Args a)
 {
-    using S = Shape<VW, NARROW>;
+    using S = Shape<VW, CUT>;
     const int lane = threadIdx.x % S::LANES;
     const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / S::LANES;
     if (unit >= a.units)
@@ -115,10 +116,10 @@ __global__ void __launch_bounds__(256) quantize_kernel(const Rows8Args a)
     }
 }
 
-template <typename T, int VW, int NARROW>
+template <typename T, int VW, int CUT>
 __global__ void __launch_bounds__(256) dequantize_kernel(const Rows8Args a)
 {
-    using S = Shape<VW, NARROW>;
+    using S = Shape<VW, CUT>;
     const int lane = threadIdx.x % S::LANES;
     const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / S::LANES;
     if (unit >= a.units)
@@ -157,15 +158,22 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const Rows8Args a)
     }
 }
 
-template <typename T, int VW, int NARROW = 32>
-cudaError_t launch(bool quantize, const Rows8Args &a, cudaStream_t st)
+template <typename T, int VW, int CUT>
+cudaError_t launch_cut(bool quantize, const Rows8Args &a, cudaStream_t st)
 {
-    const int64_t ctas = (a.units * Shape<VW, NARROW>::LANES + 255) / 256;
+    const int64_t ctas = (a.units * Shape<VW, CUT>::LANES + 255) / 256;
     if (quantize)
-        quantize_kernel<T, VW, NARROW><<<(unsigned)ctas, 256, 0, st>>>(a);
+        quantize_kernel<T, VW, CUT><<<(unsigned)ctas, 256, 0, st>>>(a);
     else
-        dequantize_kernel<T, VW, NARROW><<<(unsigned)ctas, 256, 0, st>>>(a);
+        dequantize_kernel<T, VW, CUT><<<(unsigned)ctas, 256, 0, st>>>(a);
     return cudaGetLastError();
+}
+
+template <typename T, int VW> cudaError_t launch(bool quantize, const Rows8Args &a, cudaStream_t st)
+{
+    return a.dim <= EIGHT_BLOCK / 4   ? launch_cut<T, VW, 4>(quantize, a, st)
+           : a.dim <= EIGHT_BLOCK / 2 ? launch_cut<T, VW, 2>(quantize, a, st)
+                                      : launch_cut<T, VW, 1>(quantize, a, st);
 }
 
 // Widest loads that the rows admit: 16 bytes, 8 bytes for 16-bit types, single values.
@@ -178,9 +186,7 @@ cudaError_t launch_typed(bool quantize, const Rows8Args &a, cudaStream_t st)
     if constexpr (sizeof(T) == 2)
         if (a.dim % 4 == 0 && rows_aligned(a.x, a.ld, sizeof(T), 8))
             return launch<T, 4>(quantize, a, st);
-    return a.dim <= 32   ? launch<T, 1, 8>(quantize, a, st)
-           : a.dim <= 64 ? launch<T, 1, 16>(quantize, a, st)
-                         : launch<T, 1>(quantize, a, st);
+    return launch<T, 1>(quantize, a, st);
 }
 
 int rows8_run(bool quantize, const void *x, int32_t dtype, int64_t ld, int64_t n, int32_t dim, int8_t *q, int64_t pitch,
