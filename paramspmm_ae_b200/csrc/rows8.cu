@@ -6,8 +6,8 @@
 // the result is what the formula gives in 64 bits from the two 32-bit factors.
 //
 // Bound by HBM: one pass, a lane group per block, the maximum by shuffles between the group's lanes while the values wait
-// in registers.  32,768 x 4,096 bf16: 70 us (5.8 TB/s), back 58 (7.0); 400,000 x 256 fp32: 76 us (6.8 TB/s).  Odd widths are bound by
-// their single loads and bytes: 89,251 x 47 fp32 10 us (2.3 TB/s), back 6.3.
+// in registers.  32,768 x 4,096 bf16: 70 us (5.8 TB/s), back 58 (7.0); 400,000 x 256 fp32: 84 us (6.1 TB/s).  Odd widths are bound by
+// their single loads and bytes: 89,251 x 47 fp32 8 us (2.8 TB/s), back 6.
 #include "feature_types.cuh"
 
 namespace {
@@ -23,13 +23,14 @@ struct Rows8Args {
     int32_t used;    // dim and the zeros to the next multiple of 16; bytes behind them belong to the caller
 };
 
-// LANES lanes share a block; each holds NV vectors of VW neighbouring columns, LANES * VW apart.  (Eight lanes where four do: 32,768 x 4,096
-// bf16 80 us against 70, the same divisions and shuffles for half the values.)  Rows of at most a quarter or a half of a block: CUT = 4
-// or 2, as many vectors fewer.  VW = 1, rows that are not aligned: a warp's loads and its bytes lie side by side all the same, and CUT times
-// fewer lanes do.
+// LANES lanes share a block; each holds NV vectors of VW neighbouring columns, LANES * VW apart.  CUT = 4 or 2: rows of at most a quarter or
+// a half of a block.  Few lanes with many values each take the divisions and shuffles of a scale less often, until a warp's loads
+// no longer lie side by side (to 8 bits): bf16, 32,768 x 4,096 8 lanes 80 us, 4 lanes 70, 2 lanes 96, 1,500,000 x 16 4 lanes 51, 2 lanes
+// 33; fp32, 600,000 x 64 8 lanes 43, 4 lanes 39; single values (rows that are not aligned), 100,000 x 1,001 32 lanes 125, 16 lanes 109,
+// 600,000 x 29 8 lanes 31, 4 lanes 33.
 template <int VW, int CUT> struct Shape {
-    static constexpr int LANES = VW == 8 ? 4 : VW > 1 ? 8 : 32 / CUT;
-    static constexpr int NV = VW > 1 ? EIGHT_BLOCK / (LANES * VW * CUT) : 4;
+    static constexpr int LANES = VW == 8 ? (CUT == 1 ? 4 : 2) : VW == 4 ? 4 : CUT == 1 ? 16 : 8;
+    static constexpr int NV = EIGHT_BLOCK / (LANES * VW * CUT);
 };
 
 // Unit (a row's block) of a lane group: 32-bit division where the count admits it (64-bit division was half of the odd widths' instructions).
@@ -90,14 +91,10 @@ __global__ void __launch_bounds__(256) quantize_kernel(const Rows8Args a)
         for (int i = 0; i < VW; ++i)
             most = max_nan(most, fabsf(f[v][i]));
     uint32_t top = __float_as_uint(most);
-    const uint32_t mask = S::LANES == 32 ? PSPMM_FULL_MASK : ((1u << S::LANES) - 1) << (threadIdx.x % 32 / S::LANES * S::LANES);
-    if constexpr (S::LANES == 32) {
-        top = __reduce_max_sync(mask, top);
-    } else {
+    const uint32_t mask = ((1u << S::LANES) - 1) << (threadIdx.x % 32 / S::LANES * S::LANES);
 #pragma unroll
-        for (int d = S::LANES / 2; d > 0; d >>= 1)
-            top = max(top, __shfl_xor_sync(mask, top, d));
-    }
+    for (int d = S::LANES / 2; d > 0; d >>= 1)
+        top = max(top, __shfl_xor_sync(mask, top, d));
     float scale, up;
     eight_scale(top, scale, up);
     if (lane == 0)
