@@ -3,8 +3,8 @@
 //     g = dy w [y > 0],   n = h rstd,   dx = rstd (g - n mean_j(g_j n_j)) + dh,   dw_j = sum over rows of dy_j [y > 0] n_j
 // and, where asked for, y in 8 bits (rows8.cu's form) from the same pass.
 //
-// Bound by HBM: every array is moved once.  A row is held in the registers of its lanes between the sum and its use: 8, 16 or
-// 32 lanes (several rows per warp) with up to 16 values each, a CTA of as many warps as the row needs beyond that, and two passes over a
+// Bound by HBM: every array is moved once.  A row is held in the registers of its lanes between the sum and its use: 2 to 32
+// lanes (several rows per warp) with up to 16 values each, a CTA of as many warps as the row needs beyond that, and two passes over a
 // row wider than 8,192 columns.  Rows of a CTA wait at a barrier between their sum and its use, so each asks for the row after the next
 // to be brought to L2.  x + r -> h, y in us (TB/s), alone, with y in 8 bits beside, and backward: 169,343 x 128 fp32 60 (5.8), 64, 61;
 // 16,384 x 4,096 bf16 90 (6.0), 145, 105; single values, 30,000 x 2,047 fp32 172 (5.7), 219, 186, 400,000 x 250 bf16 201 (4.0), 344, 270.  The 8-bit forms of
@@ -625,12 +625,14 @@ template <typename T, int VW, int TPR, int VPT> cudaError_t launch_backward(cons
 // the kernel: 97,235 x 144 with y in 8 bits bf16 82 -> 53 us, fp32 74 -> 57; without them bf16 43 -> 37; the backward's 24 values
 // per lane leave fewer warps, bf16 49 -> 51.
 template <bool EIGHT> struct Forward {
+    static constexpr int EIGHT_OF_FOUR = 4;
     template <int VW> static constexpr bool THREES = EIGHT || VW == 8;
     const NormArgs &a;
     cudaStream_t st;
     template <typename T, int VW, int TPR, int VPT> cudaError_t run() { return launch_forward<T, VW, TPR, VPT, EIGHT>(a, st); }
 };
 struct Backward {
+    static constexpr int EIGHT_OF_FOUR = 8;  // lanes for eight vectors of four (600,000 x 32 fp32 60 us, by four lanes 71; forward 70 in 8 bits, 61)
     template <int VW> static constexpr bool THREES = false;
     const NormBackArgs &a;
     unsigned &parts;
@@ -646,21 +648,26 @@ template <typename T, int VW, int TPR, typename L> cudaError_t three(L &l)
         return cudaErrorInvalidValue;  // (not reached)
 }
 
-// Fewest threads that hold a row in 16 values each (8 where they come singly, and less in narrow rows); false beyond 8,192 columns.
+// Fewest threads that hold a row in 16 values each (8 where they come singly); false beyond 8,192 columns.  (Eight lanes at the least, and
+// single values by 32: 1,000,000 x 16 fp32 68 us against 49, bf16 88 against 33, 600,000 x 47 fp32 154 against 82 and in 8 bits 254
+// against 113.)
 // (More would spill beside the 8-bit form's second numbers, fewer leave too few loads in flight.)
 template <typename T, int VW, typename L> bool by_width(int dim, L l, cudaError_t &e)
 {
     const int nv = (dim + VW - 1) / VW;
     if constexpr (VW == 1) {
         if (nv <= 32) e = l.template run<T, 1, 8, 4>();
-        else if (nv <= 128) e = l.template run<T, 1, 32, 4>();
+        else if (nv <= 64) e = l.template run<T, 1, 8, 8>();
+        else if (nv <= 128) e = l.template run<T, 1, 16, 8>();
         else if (nv <= 256) e = l.template run<T, 1, 32, 8>();
         else if (nv <= 1024) e = l.template run<T, 1, 128, 8>();
         else if (nv <= 4096) e = l.template run<T, 1, 512, 8>();
         else if (nv <= 8192) e = l.template run<T, 1, 1024, 8>();
         else return false;
     } else if constexpr (VW == 8) {
-        if (nv <= 8) e = l.template run<T, 8, 8, 1>();
+        if (nv <= 2) e = l.template run<T, 8, 2, 1>();
+        else if (nv <= 4) e = l.template run<T, 8, 2, 2>();
+        else if (nv <= 8) e = l.template run<T, 8, 4, 2>();
         else if (nv <= 16) e = l.template run<T, 8, 8, 2>();
         else if (L::template THREES<8> && nv <= 24) e = three<T, 8, 8>(l);
         else if (nv <= 32) e = l.template run<T, 8, 16, 2>();
@@ -672,8 +679,9 @@ template <typename T, int VW, typename L> bool by_width(int dim, L l, cudaError_
         else if (nv <= 1024) e = l.template run<T, 8, 512, 2>();
         else return false;
     } else {
-        if (nv <= 8) e = l.template run<T, VW, 8, 1>();
-        else if (nv <= 16) e = l.template run<T, VW, 8, 2>();
+        if (nv <= 4) e = l.template run<T, VW, 4, 1>();
+        else if (nv <= 8) e = l.template run<T, VW, L::EIGHT_OF_FOUR, 8 / L::EIGHT_OF_FOUR>();
+        else if (nv <= 16) e = l.template run<T, VW, 4, 4>();
         else if (L::template THREES<4> && nv <= 24) e = three<T, VW, 8>(l);
         else if (nv <= 32) e = l.template run<T, VW, 8, 4>();
         else if (L::template THREES<4> && nv <= 48) e = three<T, VW, 16>(l);

@@ -70,7 +70,7 @@ def check_forward(x, r, w, eps=1e-6, relu=False, eight=False, values=True, move=
     return h, rstd
 
 
-WIDTHS = [1, 2, 8, 16, 31, 33, 47, 64, 72, 100, 128, 130, 144, 192, 200, 250, 256, 260, 384, 500, 512, 520, 1000, 1024, 1030, 2047, 2048, 2056, 4096,
+WIDTHS = [1, 2, 8, 16, 24, 31, 32, 33, 47, 63, 64, 72, 100, 128, 130, 144, 192, 200, 250, 256, 260, 384, 500, 512, 520, 1000, 1024, 1030, 2047, 2048, 2056, 4096,
           4100, 8191, 8192, 8200, 10001]
 
 
