@@ -316,8 +316,10 @@ __global__ void __launch_bounds__(THREADS, 1) rows8_mm_kernel(const MmArgs a, co
         auto value = [&](const unsigned char *raw, int k) {
             return to_float(*reinterpret_cast<const T *>(raw + k * R::PITCH + off[k & 1] + mine));
         };
-        // x of a stage value by value, where some have no split.
+        // x of a stage value by value, where some have no split.  (Stores to TMEM are not ordered among themselves: the parts that
+        // went there before are waited for, or a NaN of theirs might land last.)
         auto store_slowly = [&](const unsigned char *raw, uint32_t to) {
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 #pragma unroll 1
             for (int k = 0; k < BK; k += 2) {
                 const float x[2] = {value(raw, k) * *reinterpret_cast<const float *>(raw + R::SCALES + k * 4),

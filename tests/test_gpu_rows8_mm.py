@@ -155,6 +155,23 @@ def test_infinities_and_nans():
     check(rows, G)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [130, 128, 47])  # rows of G on 16 bytes and off them (16 bits: 130 columns, 260 bytes)
+def test_an_infinity_in_every_stage(dtype, cols):
+    """Stages whose values have no split are stored a second time, value by value: the second store is the one that counts.  Whole
+    numbers beside one infinity per column of G, at a row of another stage each: equality, signs and NaN included."""
+    from paramspmm_ae_b200 import feature_ops as fo
+    n = 32 * cols - 5
+    rows = held(n, 300, cols, exact=True)
+    G = torch.randint(-4, 5, (n, cols), generator=torch.Generator().manual_seed(cols)).to(dtype).cuda()
+    at = (torch.arange(cols) * 32 + torch.arange(cols) * 7 % 27).cuda()
+    G[at, torch.arange(cols).cuda()] = torch.where(torch.arange(cols) % 2 == 0, float("inf"), float("-inf")).to(dtype).cuda()
+    X, inf = values(rows), float("inf")
+    want = torch.where(X[at].t() == 0, float("nan"), torch.where(X[at].t() > 0, inf, -inf)) * torch.where(torch.arange(cols).cuda() % 2 == 0, 1.0, -1.0)
+    for _ in range(4):
+        torch.testing.assert_close(fo.rows8_mm_t(rows, G), want.float(), rtol=0, atol=0, equal_nan=True)
+
+
 def test_no_rows_captured_other_streams():
     from paramspmm_ae_b200 import feature_ops as fo
     e = held(0, 40, 1)
