@@ -55,8 +55,8 @@ def _saved(ctx):
 
 
 def _held(X, eight):
-    """``X`` as the backward is to have it: itself, or in 8 bits (``eight``: True, or those bits)."""
-    return X if eight is None else feature_ops.quantize_rows(X) if eight is True else eight
+    """``X`` as the backward is to have it: itself, or in 8 bits (``eight``: True, or those bits).  ``X`` has any strides."""
+    return X if eight is None else feature_ops.quantize_rows(ops._as_rows(X)) if eight is True else eight
 
 
 class GCNFunction(torch.autograd.Function):

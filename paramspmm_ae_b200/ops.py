@@ -888,9 +888,15 @@ def dense_mm(A, B, transA=False, transB=False, out=None):
     return out
 
 
+def _as_rows(t):
+    """A matrix whose rows are stored in one piece each: ``t``, or a copy where its strides are others (the gradient of a sum,
+    a transposed view)."""
+    return t if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
 def _weight_grad(H, G):
-    """H^T G, H as a layer kept it: a tensor, or rows in 8 bits (``feature_ops.Rows8``)."""
-    return dense_mm(H, G, transA=True) if isinstance(H, torch.Tensor) else H.weight_grad(G)
+    """H^T G, H as a layer kept it: a tensor, or rows in 8 bits (``feature_ops.Rows8``).  ``G`` has any strides."""
+    return dense_mm(H, G, transA=True) if isinstance(H, torch.Tensor) else H.weight_grad(_as_rows(G))
 
 
 def dense_status():

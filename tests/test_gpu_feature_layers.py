@@ -297,3 +297,49 @@ def test_a_training_step_of_the_deep_network_is_captured():
     assert torch.equal(value, want.detach())
     for k, v in net.named_parameters():
         assert torch.equal(got[k], v.grad), k
+
+
+def _layouts(t):
+    """The same values stored by rows, by columns and as rows of a wider array."""
+    wide = torch.zeros(t.shape[0], t.shape[1] + 5, device=t.device)
+    wide[:, 3:3 + t.shape[1]] = t
+    return [t, t.t().contiguous().t(), wide[:, 3:3 + t.shape[1]]]
+
+
+@pytest.mark.parametrize("kind", ["gcn", "gcn narrow first", "gin", "agnn fused", "agnn recomputed", "agnn composed"])
+def test_gradients_and_inputs_of_any_strides_with_8_bits(kind):
+    """A layer that keeps its input in 8 bits takes what it takes without: the gradient of a sum (strides of 0), of a transposed view,
+    and inputs that are stored by columns, with equal results."""
+    from paramspmm_ae_b200 import gnn_conv
+    dev = torch.device("cuda:0")
+    g, _ = _graph(dev)
+    P = _operator(g, dev, False)
+    torch.manual_seed(6)
+    fin, fout = (12, 32) if kind == "gcn narrow first" else (36, 32)
+    layer = (gnn_conv.GINConv if kind == "gin" else gnn_conv.AGNNConv if "agnn" in kind else gnn_conv.GCNConv)(fin, fout).to(dev)
+    layer.keep_scores, layer.keep_input_8bit = kind != "agnn recomputed", True
+    args = (P.colIdx.unsqueeze(-1),) if "agnn" in kind else ()
+    X, G = torch.randn(g.n_rows, fin, device=dev), torch.randn(g.n_rows, fout, device=dev)
+    fused, gnn_conv.FUSE_AGNN_TRAINING = gnn_conv.FUSE_AGNN_TRAINING, kind != "agnn composed"
+    old, gnn_conv.REORDER_NARROW_FIRST = gnn_conv.REORDER_NARROW_FIRST, kind == "gcn narrow first"
+
+    def step(x, back):
+        layer.zero_grad()
+        x = x.detach().requires_grad_(True)
+        out = layer(x, {fin: P, fout: P}, *args)
+        back(out)
+        return out.detach(), x.grad, layer.weights.grad
+
+    try:
+        want = step(X, lambda out: out.backward(G))
+        for x in _layouts(X)[1:] if kind != "gin" else ():  # (the aggregation of GIN itself takes contiguous rows alone)
+            for a, b in zip(step(x, lambda out: out.backward(G)), want):
+                _close(a, b)
+        for grad in _layouts(G)[1:]:
+            for a, b in zip(step(X, lambda out: out.backward(grad)), want):
+                _close(a, b)
+        ones = step(X, lambda out: out.backward(torch.ones_like(G)))
+        for a, b in zip(step(X, lambda out: out.sum().backward()), ones):
+            _close(a, b)
+    finally:
+        gnn_conv.FUSE_AGNN_TRAINING, gnn_conv.REORDER_NARROW_FIRST = fused, old
