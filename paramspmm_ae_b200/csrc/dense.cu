@@ -940,12 +940,4 @@ extern "C" int pspmm_dense_mm_stalled(int32_t transA, int32_t transB, int64_t M,
     return dense_run(transA, transB, M, N, K, A, ldA, B, ldB, C, ldC, scratch, scratch_bytes, 20000000u, 1, stream);
 }
 
-extern "C" int pspmm_dense_status(int32_t *status)
-{
-    if (!status)
-        return PSPMM_E_ARG;
-    unsigned v = 0;
-    PSPMM_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_dense_status, sizeof(v)));
-    *status = (int32_t)v;
-    return PSPMM_OK;
-}
+extern "C" int pspmm_dense_status(int32_t *status) { return pspmm_read_status(g_dense_status, status); }

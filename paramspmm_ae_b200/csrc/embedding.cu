@@ -791,12 +791,4 @@ extern "C" int pspmm_embedding_grad(const void *ids, int32_t ids64, int64_t n, c
     return PSPMM_OK;
 }
 
-extern "C" int pspmm_embedding_status(int32_t *status)
-{
-    if (!status)
-        return PSPMM_E_ARG;
-    unsigned v = 0;
-    PSPMM_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_embedding_status, sizeof(v)));
-    *status = (int32_t)v;
-    return PSPMM_OK;
-}
+extern "C" int pspmm_embedding_status(int32_t *status) { return pspmm_read_status(g_embedding_status, status); }

@@ -203,15 +203,7 @@ extern "C" int pspmm_pull_rows_bulk(const pspmm_row_sources *sources, const int3
     return pull_rows_impl(sources, rows, n, dst, dim, ld_src, ld_dst, rotate, ctas, stream, true);
 }
 
-extern "C" int pspmm_pull_rows_status(int32_t *status)
-{
-    if (!status)
-        return PSPMM_E_ARG;
-    int v = 0;
-    PSPMM_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_pull_status, sizeof(int)));
-    *status = v;
-    return PSPMM_OK;
-}
+extern "C" int pspmm_pull_rows_status(int32_t *status) { return pspmm_read_status(g_pull_status, status); }
 
 namespace {
 

@@ -23,6 +23,19 @@ int pspmm_note_cuda_error(cudaError_t e);
             return pspmm_note_cuda_error(e__);  \
     } while (0)
 
+// Host side: a status word of the current GPU, after the work that is queued there on any stream.  (A copy alone waits for the default
+// stream, and not for those that do not wait for it.)
+template <typename T> static inline int pspmm_read_status(const T &word, int32_t *status)
+{
+    if (!status)
+        return PSPMM_E_ARG;
+    T v = 0;
+    PSPMM_CUDA_TRY(cudaDeviceSynchronize());
+    PSPMM_CUDA_TRY(cudaMemcpyFromSymbol(&v, word, sizeof(v)));
+    *status = (int32_t)v;
+    return PSPMM_OK;
+}
+
 // Programmatic dependent launch: a kernel launched with launch_dependent() may start while the
 // kernel before it on the stream drains; what it must not do before pdl_wait() is touch memory that
 // kernel writes.  A kernel calls pdl_launch_dependents() once its CTAs are placed.  Both are no-ops

@@ -739,12 +739,4 @@ extern "C" int pspmm_rows8_mm_t_stalled(const int8_t *q, int64_t pitch, const fl
     return mm_run(q, pitch, scales, n, dim, G, dtype, ldG, cols, C, ldC, scratch, scratch_bytes, 20000000u, 1, stream);
 }
 
-extern "C" int pspmm_rows8_mm_status(int32_t *status)
-{
-    if (!status)
-        return PSPMM_E_ARG;
-    unsigned v = 0;
-    PSPMM_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_rows8_mm_status, sizeof(v)));
-    *status = (int32_t)v;
-    return PSPMM_OK;
-}
+extern "C" int pspmm_rows8_mm_status(int32_t *status) { return pspmm_read_status(g_rows8_mm_status, status); }

@@ -343,3 +343,40 @@ def test_gradients_and_inputs_of_any_strides_with_8_bits(kind):
             _close(a, b)
     finally:
         gnn_conv.FUSE_AGNN_TRAINING, gnn_conv.REORDER_NARROW_FIRST = fused, old
+
+
+@pytest.mark.parametrize("which", ["embedding", "rows8_mm", "dense"])
+def test_status_words_wait_for_every_stream(which):
+    """A status read while the call that sets it waits its turn on a side stream, in a process of its own (the words stay set)."""
+    import subprocess
+    import sys
+    code = """
+import ctypes, sys, torch
+from paramspmm_ae_b200 import _lib, feature_ops as fo, ops
+which = sys.argv[1]
+lib, side = _lib.lib(), torch.cuda.Stream()
+status = {"embedding": fo.embedding_status, "rows8_mm": fo.rows8_mm_status, "dense": ops.dense_status}[which]
+table, ids = torch.ones(4, 8, device="cuda"), torch.tensor([0, 4], device="cuda")
+q, s, G = torch.ones(400, 64, dtype=torch.int8, device="cuda"), torch.ones(400, 1, device="cuda"), torch.ones(400, 32, device="cuda")
+A, C, scratch = torch.ones(400, 64, device="cuda"), torch.zeros(64, 32, device="cuda"), torch.zeros(1 << 22, dtype=torch.uint8, device="cuda")
+def stalled(of):
+    at = torch.cuda.current_stream().cuda_stream
+    if of == "rows8_mm":
+        _lib.check(lib.pspmm_rows8_mm_t_stalled(q.data_ptr(), 64, s.data_ptr(), 400, 64, G.data_ptr(), 0, 32, 32, C.data_ptr(), 32,
+                                                scratch.data_ptr(), 1 << 22, at))
+    else:
+        _lib.check(lib.pspmm_dense_mm_stalled(1, 0, 64, 32, 400, A.data_ptr(), 64, G.data_ptr(), 32, C.data_ptr(), 32,
+                                              scratch.data_ptr(), 1 << 22, at))
+fo.embedding(ids[:1], table)
+fo.rows8_mm_t(fo.Rows8(q, s, 64), G)
+ops.dense_mm(A, G, transA=True)
+torch.cuda.synchronize()
+assert status() == 0
+with torch.cuda.stream(side):
+    torch.cuda._sleep(100000000)  # some 50 ms
+    fo.embedding(ids, table) if which == "embedding" else stalled(which)
+assert status() == 1
+print("told")
+"""
+    p = subprocess.run([sys.executable, "-c", code, which], capture_output=True, text=True, timeout=120)
+    assert p.returncode == 0 and "told" in p.stdout, p.stderr
