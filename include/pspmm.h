@@ -429,7 +429,8 @@ PSPMM_API int pspmm_rows8_mm_status(int32_t *status);
  *     h = x + residual,   rstd = (mean(h^2) + eps)^-1/2,   y = h * rstd * weight   (relu != 0: negative y become 0)
  * residual may be NULL (h = x).  h and y may each be NULL: not wanted.  rstd[n] is always written.  q / scales (both or
  * neither): y in the 8-bit form above, from h, rstd and y with twice the bits of 32-bit ones; y and h are the same with and
- * without it.  No output may overlap an input.
+ * without it.  No output may overlap an input.  A row below 2^-128 with eps = 0 has no 32-bit rstd (it becomes an infinity, as for a
+ * row of zeros), and no y of use.
  * Backward, from h as stored and rstd:  with g = dy * weight (0 where relu cut) and m = h * rstd,
  *     dx = rstd * (g - m * mean(g * m)) + dh   (the gradient of x and of residual; dh, the one that reaches h itself, may be NULL)
  *     dweight = sum over rows of dy * m (0 where relu cut), in an order that depends on the sizes alone.

@@ -268,8 +268,11 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST, ctas_for(TPR, VW * VPT, EIGHT
         }
         if constexpr (EIGHT) {
             // (h + low) rstd w as a sum of two 32-bit numbers, the first the sum rounded: products and what their rounding leaves (fma).
-            const float rest = (float)(rstd64 - rstd);
-            const pair_t by = make_pair(rstd, rstd), by_less = make_pair(-rstd, -rstd), by_rest = make_pair(rest, rest);
+            // A row whose rstd is no number (NaN, or infinite) takes 0 in its place, so that the columns behind it stay zeros, and a NaN
+            // among the magnitudes of each block.
+            const bool number = rstd < __int_as_float(0x7f800000);
+            const float by1 = number ? rstd : 0.f, rest = number ? (float)(rstd64 - rstd) : 0.f, none = number ? 0.f : __int_as_float(0x7fc00000);
+            const pair_t by = make_pair(by1, by1), by_less = make_pair(-by1, -by1), by_rest = make_pair(rest, rest);
 #pragma unroll
             for (int e = 0; e < VALUES; e += 2) {
                 const pair_t x = pair_of(h, e), f = pair_of(w, e), n = mul_pair(x, by), less_n = mul_pair(x, by_less);
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(Rows<TPR>::MOST, ctas_for(TPR, VW * VPT, EIGHT
             int8_t *q = a.q + row * a.pitch;
 #pragma unroll
             for (int v0 = 0; v0 < VPT; v0 += SB) {
-                float most = 0.f;
+                float most = none;
 #pragma unroll
                 for (int v = v0; v < v0 + SB && v < VPT; ++v)
 #pragma unroll

@@ -298,3 +298,18 @@ def test_refusals():
                 lambda: fo.rms_norm_backward(x, x, torch.ones(6, device="cuda").double(), w)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 36), (torch.float32, 47), (torch.float32, 100), (torch.float32, 4100), (torch.float32, 8200),
+                                       (torch.bfloat16, 24), (torch.bfloat16, 100), (torch.bfloat16, 250), (torch.bfloat16, 2056), (torch.float16, 4101)])
+def test_columns_behind_rows_of_nan_are_zeros_in_8_bits(dtype, dim):
+    """The columns from dim to the next multiple of 16, whatever the row holds."""
+    from paramspmm_ae_b200 import feature_ops as fo
+    x, r, w = inputs(9, dim, dtype, 31)
+    x[0, 0], x[1, dim - 1], x[2, dim // 2] = float("nan"), float("nan"), float("inf")
+    x[3], r[3] = 0, 0
+    x[4] = float("nan")
+    for eps in (1e-6, 0.0):
+        for relu in (False, True):
+            kept = fo.rms_norm(x.cuda(), w.cuda(), r.cuda(), eps=eps, relu=relu, eight_bit=True)[3]
+            assert kept.q.shape[1] == (dim + 15) // 16 * 16 and not kept.q[:, dim:].any()
