@@ -97,6 +97,33 @@ def test_one_id_takes_everything(n):
         check_grad(ids.flip(0).contiguous(), G, V)
 
 
+def chunk_length(n):
+    """Positions of a chunk of the gradient, from the pieces that its scratch has room for: two rows per chunk."""
+    import ctypes
+    from paramspmm_ae_b200 import _lib
+    need = [ctypes.c_size_t(0) for _ in range(2)]
+    for dim, c in zip((64, 128), need):  # (multiples of the 256 bytes that parts of the scratch are rounded to)
+        _lib.check(_lib.lib().pspmm_embedding_grad_scratch_bytes(n, dim, ctypes.byref(c)))
+    chunks = (need[1].value - need[0].value) // (2 * 64 * 4)
+    return next(run for run in (2 ** i for i in range(12)) if (n + run - 1) // run == chunks)
+
+
+@pytest.mark.parametrize("n,dim", [(2048, 20), (4096, 130), (4097, 47), (65536, 20), (65537, 130), (262145, 20), (1048576, 8), (1048577, 3)])
+def test_runs_around_the_length_of_chunks(n, dim):
+    """Runs one shorter and longer than a chunk, than a few, and than the 64 from which on a CTA of its own adds the pieces, that
+    begin with a chunk and inside one.  Whole numbers: equality."""
+    from paramspmm_ae_b200 import feature_ops as fo
+    run = chunk_length(n)
+    G = torch.randint(-4, 5, (n, dim), generator=torch.Generator().manual_seed(n)).float().cuda()
+    for chunks in (1, 2, 3, 63, 64, 65, 66):
+        for length in (chunks * run - 1, chunks * run, chunks * run + 1):
+            for before in (0, 1, run // 2, run - 1, run + 3):
+                ids = torch.div(torch.arange(n, device="cuda") + length - before % length, length, rounding_mode="floor")
+                V = int(ids[-1]) + 2
+                want = torch.zeros(V, dim, device="cuda").index_add_(0, ids, G)  # (whole numbers below 2^24 in any order)
+                assert torch.equal(fo.embedding_grad(ids, G, V), want), (length, before)
+
+
 @pytest.mark.parametrize("V", [1, 2, 255, 256, 257, 511, 512, 65535, 65536, 65537, 131072, 262143, 262144, 16777217])
 @pytest.mark.parametrize("n", [3001, 70001])
 def test_table_sizes(V, n):
