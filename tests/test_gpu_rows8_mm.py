@@ -102,6 +102,22 @@ def test_no_bias_over_a_long_sum():
     assert ((got - want).abs() / want).max() <= 64 * U
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,cols", [(47, 8), (130, 130)])
+@pytest.mark.parametrize("n", [1, 32, 63, 64, 65, 128, 129, 1000, 10007, 100003])
+def test_chains_as_they_are(dtype, dim, cols, n):
+    """The bound from the chains that the kernel runs, on values of one sign, where truncations agree: two stages of 32 rows, of each
+    three parts in two instructions, so 12 truncating additions (24 u S) per 64 rows; scale * G is rounded once (u S); then one addition
+    per chain, and over at most 592 ranges of rows 19 + 3 + 2 + 7 in sequence.  Together less than (n / 64 + 60) u S."""
+    from paramspmm_ae_b200 import feature_ops as fo
+    g = torch.Generator(device="cuda").manual_seed(n + dim)
+    rows = fo.Rows8(torch.randint(1, 128, (n, (dim + 15) // 16 * 16), generator=g, device="cuda").to(torch.int8),
+                    torch.rand(n, (dim + 127) // 128, generator=g, device="cuda") + 0.01, dim)
+    G = (torch.rand(n, cols, generator=g, device="cuda") + 1e-3).to(dtype)
+    got, want = fo.rows8_mm_t(rows, G).double(), values(rows).t() @ G.double()
+    assert ((got - want).abs() <= (n / 64 + 60) * U * want).all(), ((got - want).abs() / want).max().item() / U
+
+
 def test_rows_quantised_here_and_views():
     from paramspmm_ae_b200 import feature_ops as fo
     g = torch.Generator(device="cuda").manual_seed(2)
