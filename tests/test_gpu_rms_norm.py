@@ -313,3 +313,29 @@ def test_columns_behind_rows_of_nan_are_zeros_in_8_bits(dtype, dim):
         for relu in (False, True):
             kept = fo.rms_norm(x.cuda(), w.cuda(), r.cuda(), eps=eps, relu=relu, eight_bit=True)[3]
             assert kept.q.shape[1] == (dim + 15) // 16 * 16 and not kept.q[:, dim:].any()
+
+
+def rows_between_two_roundings(n, dim, dtype, seed):
+    """Rows whose (mean h^2)^-1/2 lies, as far as 64 bits tell, half way between two 32-bit numbers: the order in which the squares are
+    added decides which of the two it becomes."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, dim, generator=g).to(dtype).double()
+    x[:, -8:] = 0
+    near = x.square().mean(-1).mul(1.0001).rsqrt().float()
+    half_way = (near.double() + torch.nextafter(near, torch.zeros_like(near)).double()) / 2
+    want = half_way.pow(-2) * dim
+    for c in range(dim - 8, dim):  # what is missing, as far as one more value can give it
+        x[:, c] = (want - x.square().sum(-1)).clamp(min=0).sqrt().mul(1 - 2.0 ** -12 if c < dim - 1 else 1).to(dtype).double()
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [24, 68, 96, 132, 144, 192, 260, 300, 384, 1000, 2056])
+def test_the_8_bit_form_leaves_the_other_outputs_alone(dtype, dim):
+    from paramspmm_ae_b200 import feature_ops as fo
+    x = rows_between_two_roundings(30000, dim, dtype, dim).cuda()
+    w, r = torch.ones(dim, dtype=dtype, device="cuda"), torch.zeros_like(x)
+    for residual in (None, r):
+        y, h, rstd, _ = fo.rms_norm(x, w, residual, eps=0.0)
+        y8, h8, rstd8, _ = fo.rms_norm(x, w, residual, eps=0.0, eight_bit=True)
+        assert torch.equal(h, h8) and torch.equal(rstd, rstd8) and torch.equal(y, y8), (rstd != rstd8).sum().item()
