@@ -433,7 +433,8 @@ PSPMM_API int pspmm_rows8_mm_status(int32_t *status);
  * row of zeros), and no y of use.
  * Backward, from h as stored and rstd:  with g = dy * weight (0 where relu cut) and m = h * rstd,
  *     dx = rstd * (g - m * mean(g * m)) + dh   (the gradient of x and of residual; dh, the one that reaches h itself, may be NULL)
- *     dweight = sum over rows of dy * m (0 where relu cut), in an order that depends on the sizes alone.
+ *     dweight = sum over rows of dy * m (0 where relu cut), in an order that depends on the sizes, the type, on which bytes the
+ *               operands' rows begin, and on the GPU: equal calls give equal bits, copies at other places need not.
  * dx may be dh.  Scratch: pspmm_rms_norm_backward_scratch_bytes, 4-byte aligned.  n == 0 gives a dweight of zeros.
  */
 PSPMM_API int pspmm_rms_norm(const void *x, int64_t ld_x, const void *residual, int64_t ld_residual, const void *weight,
