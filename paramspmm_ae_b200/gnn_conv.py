@@ -278,7 +278,7 @@ class RMSNormFunction(torch.autograd.Function):
 
 class NodeEmbedding(torch.nn.Module):
     """Learned features: ``scale * weights[ids]`` for graphs whose nodes have none.  ``padding_idx`` names a row that takes no
-    gradient (ids that fill up a batch)."""
+    gradient (ids that fill up a batch).  ``ids``: int32 or int64 on the weights' GPU, of any shape and strides."""
 
     def __init__(self, n_rows, dim, scale=1.0, padding_idx=None):
         super().__init__()
@@ -295,7 +295,7 @@ class NodeEmbedding(torch.nn.Module):
             self.weights.data[self.padding_idx] = 0
 
     def forward(self, ids):
-        return EmbeddingFunction.apply(ids, self.weights, self.scale, self.padding_idx)
+        return EmbeddingFunction.apply(ids.contiguous() if isinstance(ids, torch.Tensor) else ids, self.weights, self.scale, self.padding_idx)
 
 
 class RMSNorm(torch.nn.Module):
@@ -305,7 +305,9 @@ class RMSNorm(torch.nn.Module):
         y, h, kept = norm(conv_out, h, eight_bit=True)
         conv_out = conv(y, spmm_dict, kept)   # the layer keeps those 8 bits for its backward instead of y
 
-    The backward keeps h, so that with relu in here and the next layer's input in 8 bits nothing else of this step lives on."""
+    The backward keeps h, so that with relu in here and the next layer's input in 8 bits nothing else of this step lives on.
+    ``x`` and ``residual`` have one shape, any strides (other than rows are copied), and the weights' type: float32, or what
+    ``.to`` has made of it."""
 
     def __init__(self, dim, eps=1e-6, relu=False):
         super().__init__()
@@ -313,6 +315,7 @@ class RMSNorm(torch.nn.Module):
         self.weights = torch.nn.Parameter(torch.ones(dim))
 
     def forward(self, x, residual=None, eight_bit=False):
+        x, residual = (ops._as_rows(t) if isinstance(t, torch.Tensor) else t for t in (x, residual))
         y, h, q, scales = RMSNormFunction.apply(x, residual, self.weights, self.eps, self.relu, eight_bit)
         h = x if residual is None else h
         return (y, h, feature_ops.Rows8(q, scales, x.shape[-1], x.shape)) if eight_bit else (y, h)

@@ -380,3 +380,36 @@ print("told")
 """
     p = subprocess.run([sys.executable, "-c", code, which], capture_output=True, text=True, timeout=120)
     assert p.returncode == 0 and "told" in p.stdout, p.stderr
+
+
+def test_node_embedding_and_norm_take_any_strides():
+    """Ids that are a column of a batch, activations that are stored by columns or that repeat one row: equal to their copies."""
+    from paramspmm_ae_b200 import gnn_conv
+    torch.manual_seed(7)
+    layer = gnn_conv.NodeEmbedding(50, 24).cuda()
+    batch = torch.randint(0, 50, (40, 6), device="cuda")
+    for ids in (batch[:, 2], batch.t(), batch[::3, 1::2], batch[0, 0], batch[:1].expand(5, 6)):
+        got = []
+        for i in (ids, ids.clone(memory_format=torch.contiguous_format)):
+            layer.zero_grad()
+            out = layer(i)
+            out.square().sum().backward()
+            got.append((out.detach(), layer.weights.grad))
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and torch.equal(got[0][0], layer.weights[ids])
+    norm = gnn_conv.RMSNorm(70).cuda()
+    norm.weights.data.uniform_(0.5, 1.5)
+    base, res = torch.randn(70, 33, device="cuda"), torch.randn(1, 70, device="cuda")
+    wide = torch.randn(4, 33, 75, device="cuda")
+    for x, r in ((base.t(), None), (base.t(), res.expand(33, 70)), (res.expand(33, 70), base.t()), (wide[:, :, 2:72], None),
+                 (wide[1, :, 2:72], base.t())):
+        got = []
+        for copy in (False, True):
+            norm.zero_grad()
+            a, b = ((t if t is None else (t.clone(memory_format=torch.contiguous_format) if copy else t.detach()).requires_grad_(True)) for t in (x, r))
+            y, h, kept = norm(a, b, eight_bit=True)
+            (y * h).square().sum().backward()
+            got.append([y.detach(), h.detach(), kept.q, a.grad, norm.weights.grad] + ([] if b is None else [b.grad]))
+        _close(got[0][0], got[1][0])
+        assert torch.equal(got[0][1], got[1][1]) and (got[0][2] != got[1][2]).sum() == 0
+        for p, q in zip(got[0][3:], got[1][3:]):
+            torch.testing.assert_close(p, q, rtol=1e-5, atol=1e-4 * float(q.abs().max()))
