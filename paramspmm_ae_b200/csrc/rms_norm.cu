@@ -4,11 +4,11 @@
 // and, where asked for, y in 8 bits (rows8.cu's form) from the same pass.
 //
 // Bound by HBM: every array is moved once.  A row is held in the registers of its lanes between the sum and its use: 2 to 32
-// lanes (several rows per warp) with up to 16 values each, a CTA of as many warps as the row needs beyond that, and two passes over a
+// lanes (several rows per warp) with up to 24 values each (16 in the backward), a CTA of as many warps as the row needs beyond that, and two passes over a
 // row wider than 8,192 columns.  Rows of a CTA wait at a barrier between their sum and its use, so each asks for the row after the next
 // to be brought to L2.  x + r -> h, y in us (TB/s), alone, with y in 8 bits beside, and backward: 169,343 x 128 fp32 60 (5.8), 64, 61;
 // 16,384 x 4,096 bf16 90 (6.0), 145, 105; single values, 30,000 x 2,047 fp32 172 (5.7), 219, 186, 400,000 x 250 bf16 201 (4.0), 344, 270.  The 8-bit forms of
-// wide rows are bound by instructions: 43 per value and thread, 56 % of issue slots.  (Measured and left: rows brought to shared memory by bulk copies, several in
+// wide rows are bound by instructions: 43 per value and thread, 57 % of issue slots.  (Measured and left: rows brought to shared memory by bulk copies, several in
 // flight per CTA, one more pass of instructions over every value, bf16 127, 210, 159; second numbers for the values next to a half
 // and the largest ones alone, from memory again, which was 15 % slower than all of them from registers.)
 //
@@ -651,7 +651,7 @@ template <typename T, int VW, int TPR, typename L> cudaError_t three(L &l)
         return cudaErrorInvalidValue;  // (not reached)
 }
 
-// Fewest threads that hold a row in 16 values each (8 where they come singly); false beyond 8,192 columns.  (Eight lanes at the least, and
+// Fewest threads that hold a row in 16 values each (8 where they come singly, 24 by THREES of eight); false beyond 8,192 columns.  (Eight lanes at the least, and
 // single values by 32: 1,000,000 x 16 fp32 68 us against 49, bf16 88 against 33, 600,000 x 47 fp32 154 against 82 and in 8 bits 254
 // against 113.)
 // (More would spill beside the 8-bit form's second numbers, fewer leave too few loads in flight.)

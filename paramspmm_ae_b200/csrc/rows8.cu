@@ -197,7 +197,7 @@ int rows8_run(bool quantize, const void *x, int32_t dtype, int64_t ld, int64_t n
         return PSPMM_E_ARG;
     const int64_t blocks = ((int64_t)dim + EIGHT_BLOCK - 1) / EIGHT_BLOCK;
     const int64_t units = n * blocks;
-    if (pitch > INT32_MAX || dim > INT32_MAX - 8192 || n > ((int64_t)INT32_MAX * 8) / blocks)  // CTAs of eight blocks
+    if (pitch > INT32_MAX || dim > INT32_MAX - 8192 || n > ((int64_t)INT32_MAX * 8) / blocks)  // (a CTA takes 16 at least)
         return PSPMM_E_RANGE;
     Rows8Args a = {x, q, scales, n, ld, units, dim, (int32_t)pitch, (int32_t)blocks, (dim + 15) / 16 * 16};
     cudaError_t e = dtype == PSPMM_F32    ? launch_typed<float>(quantize, a, (cudaStream_t)stream)

@@ -22,8 +22,9 @@
 // partial tiles in scratch, which reduce_kernel adds in order.  G with unaligned rows is copied to aligned ones first where scratch
 // has room for it.
 //
-// Bound by the loading warps' instructions: 2,270 per stage of a tile are issued in 900 cycles (67 % of the slots), of which cutting x takes
-// 4 x 180 and unpacking q 4 x 85; the MMAs take 384 of those cycles, DRAM stands at a third.  2,449,029 x 256 x 256 fp32: 1,075 us (1,265 in
+// No unit is full: of the issue slots, the fullest, 68 % are taken in active cycles, the tensor pipe stands at 46 %, DRAM at a third.  2,270
+// instructions per stage of a tile are issued in 900 cycles, of which the MMAs take 384; cutting x takes 4 x 180 of the instructions and
+// unpacking q 4 x 85, the other half, waits, copies and the adding up of chains, has not been broken down.  2,449,029 x 256 x 256 fp32: 1,075 us (1,265 in
 // long runs under the power cap) against 600 for the MMAs and 480 for the bytes; one loading group that takes its rows through registers
 // 1,926.  19,717 x 500 x 16: 20 us, start and the adding of partial tiles.  The copy of unaligned rows: 1,029,577 x 285 fp16 314 us.
 //
