@@ -407,7 +407,8 @@ PSPMM_API int pspmm_dequantize_rows(const int8_t *q, int64_t pitch, const float 
 /*
  * C[dim, cols] = X^T G, fp32, where X[n, dim] is held in the 8-bit form (q, scales) and G[n, cols] has element type dtype: the weight
  * gradient of a layer that kept its input in 8 bits.  On the tensor cores with fp32 accuracy: q is exact in bf16, scale * G (rounded
- * to fp32) is cut into three bf16 parts whose sum it is.  Any size and alignment of G.  Scratch, 16-byte aligned:
+ * to fp32) is cut into three bf16 parts whose sum it is.  (Where that product leaves fp32 it is an infinity, and a q of 0 beside it gives
+ * NaN.)  Any size and alignment of G.  Scratch, 16-byte aligned:
  * pspmm_rows8_mm_t_scratch_bytes(n, dim, cols, dtype, 1) bytes are required; aligned = 0, for a G whose rows do not all start on 16
  * bytes, adds room for a copy of G whose rows do, without which such a product takes two to three times as long.  n == 0 gives
  * zeros.  Waits inside the kernel are bounded (two
