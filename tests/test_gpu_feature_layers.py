@@ -413,3 +413,43 @@ def test_node_embedding_and_norm_take_any_strides():
         assert torch.equal(got[0][1], got[1][1]) and (got[0][2] != got[1][2]).sum() == 0
         for p, q in zip(got[0][3:], got[1][3:]):
             torch.testing.assert_close(p, q, rtol=1e-5, atol=1e-4 * float(q.abs().max()))
+
+
+def test_offsets_beyond_32_bits():
+    """Arrays of more than 2^31 values (4.4 GB each): the rows at their ends are what they are in arrays of their own."""
+    from paramspmm_ae_b200 import feature_ops as fo
+    n, dim, m = 16600000, 130, 999
+    assert n * dim > 2 ** 31 and (n - m) * dim > 2 ** 31
+    g = torch.Generator(device="cuda").manual_seed(8)
+    end = torch.randint(-4, 5, (m, dim), generator=g, device="cuda").bfloat16()
+    x = torch.zeros(n, dim, dtype=torch.bfloat16, device="cuda")
+    x[-m:] = end
+    w = torch.rand(dim, generator=g, device="cuda").bfloat16()
+    alone, whole = fo.rms_norm(end, w, end, eight_bit=True), fo.rms_norm(x, w, x, eight_bit=True)
+    for a, b in zip(alone[:3] + (alone[3].q, alone[3].scales), whole[:3] + (whole[3].q, whole[3].scales)):
+        assert torch.equal(a, b[-m:]) and b.shape[0] == n
+    assert torch.equal(alone[3].dequantize(torch.bfloat16), whole[3].dequantize(torch.bfloat16)[-m:])
+    a, b = (fo.rms_norm_backward(t, s[1], s[2], w, dh=t) for t, s in ((end, alone), (x, whole)))
+    assert torch.equal(a[0], b[0][-m:])
+    torch.testing.assert_close(b[1].float(), a[1].float(), rtol=2 ** -7, atol=1e-2)  # (rows of zeros add none; other partial sums)
+    del whole, b
+    held, kept = fo.quantize_rows(end), fo.quantize_rows(x)
+    assert torch.equal(held.q, kept.q[-m:]) and torch.equal(held.scales, kept.scales[-m:])
+    kept = fo.Rows8(kept.q, kept.scales.fill_(0.5), dim)  # (products of whole numbers and halves: exact)
+    held = fo.Rows8(held.q, held.scales.fill_(0.5), dim)
+    want = (held.q[:, :dim].double() * 0.5).t() @ end.double()
+    assert torch.equal(fo.rows8_mm_t(held, end).double(), want) and torch.equal(fo.rows8_mm_t(kept, x).double(), want)
+    wide = torch.zeros(n, 132, dtype=torch.bfloat16, device="cuda")  # rows that begin off 16 bytes, and no room needed for a copy of them
+    wide[-m:, 1:131] = end
+    assert torch.equal(fo.rows8_mm_t(kept, wide[:, 1:131]).double(), want)
+    del kept, wide
+    ids = torch.randperm(m, generator=g, device="cuda")
+    assert torch.equal(fo.embedding(ids + (n - m), x), end[ids])
+    grad = fo.embedding_grad(ids + (n - m), end, n)
+    assert torch.equal(grad[-m:][ids], end) and not grad[:-m].any()
+    del grad
+    ids = torch.cat([torch.full((n - m,), 3, device="cuda"), ids + 10])
+    table = torch.randn(m + 10, dim, generator=g, device="cuda").bfloat16()
+    assert torch.equal(fo.embedding(ids, table)[-m:], table[ids[-m:]])
+    grad = fo.embedding_grad(ids, x, m + 10)
+    assert torch.equal(grad[ids[-m:]], end) and not grad[:10].any()
